@@ -93,7 +93,18 @@ constexpr size_t kSmem = 1024 + (size_t)STAGES * kStage + kOutSmem + 512;
 // tmH over gu = [u | g]) one chunk ahead into two staging slots and writes
 // du = dh silu(g) and dg = dh u s (1 + g (1 - s)), s = sigmoid(g), through tmC
 // and tmG (dgu = [du | dg]) from the same slots; dh itself never reaches memory.
-enum Epi : int { kStore = 0, kAccumF32 = 1, kSwiGLU = 2, kRoPE = 3, kAxpby = 4, kSwiGLUBwd = 5 };
+// kLse: the language-model head in the forward of the softmax cross entropy.  The
+// logits stay in tensor memory: each epilogue thread walks over the 256 logits of
+// its row in the tile with a running maximum m and a running sum of
+// 2^((z - m) log2 e), writes that pair to args.part[tile column][row], and the
+// logit of the row's target, where the tile holds it, to args.target_logit.
+// kCeGrad: the same product again in the backward: with the row's statistics
+// (m, log2 sum) over the whole vocabulary the tile becomes
+// (softmax(z) - onehot(target)) * args.row_scale[row], rounded to the operand type
+// of the two gradient products, and goes out through tmC.
+enum Epi : int {
+  kStore = 0, kAccumF32 = 1, kSwiGLU = 2, kRoPE = 3, kAxpby = 4, kSwiGLUBwd = 5, kLse = 6, kCeGrad = 7
+};
 
 struct PairArgs {
   void* C;
@@ -117,6 +128,18 @@ struct PairArgs {
   // Pipeline trace (null in normal runs): %globaltimer stamps of the first
   // kTraceUnits work units of CTA pair 0, layout [event][unit].
   unsigned long long* trace;
+  // A factor of C in device memory (null: 1); TMA epilogues of kStore only.
+  const float* alpha_dev;
+  // With splits > 1: every K range has its own matrix of C (the third coordinate of
+  // tmC), so the partial sums meet in an order that the caller chooses.
+  int split_c;
+  // kLse / kCeGrad only; targets are full-vocabulary ids, col0 the first of B's rows
+  const int64_t* targets;
+  int64_t col0;
+  float2* part;
+  float* target_logit;
+  const float2* stats;
+  const float* row_scale;
 };
 
 constexpr int kTraceUnits = 64;
@@ -402,6 +425,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     constexpr int kSlots = (int)(kOutWarpBytes / kBox);         // 2 (fp32) or 4 (16-bit)
     int acc = 0, nbox = 0;
     uint32_t acc_phase = 0, dpar = 0;
+    const float alpha = args.alpha_dev != nullptr ? args.alpha * __ldg(args.alpha_dev) : args.alpha;
     for (int unit = pair; unit < num_units; unit += npairs) {
       int tm, tn, kb0, kb1, bi;
       unit_coords(unit, num_tiles, tiles_m, tiles_n, nk, args, tm, tn, kb0, kb1, bi);
@@ -664,6 +688,96 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         if (++acc == 2) { acc = 0; acc_phase ^= 1; }
         continue;
       }
+      if constexpr (EPI == kLse || EPI == kCeGrad) {
+        const int row = row0 + lane;
+        const bool in = row < args.M;
+        // the target's column in this product, -1 where it has none
+        const int64_t t64 = in ? __ldg(args.targets + row) - args.col0 : -1;
+        const int target = t64 >= 0 && t64 < args.N ? (int)t64 : -1;
+        float m = -INFINITY, s = 0.f, scale = 0.f;
+        if constexpr (EPI == kCeGrad) {
+          if (in) {
+            const float2 st = __ldg(args.stats + row);
+            m = st.x;
+            s = st.y;
+            scale = __ldg(args.row_scale + row);
+          }
+        }
+#pragma unroll 1
+        for (int c = 0; c < BN / 32; ++c) {
+          uint32_t r[32];
+          tmem_ld_32x32b_x32(tmem + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * BN + c * 32), r);
+          tmem_ld_wait();
+          if (c == BN / 32 - 1) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_addr(&accempty[acc]), 0));
+            if (tracer) trace_unit(args, kTrEpiFreed, ui);
+          }
+          const int col0 = tn * BN + c * 32;
+          if (row0 >= args.M || col0 >= args.N) continue;
+          const int tj = target - col0;  // in [0, 32) where this chunk holds the target
+          const bool here = __any_sync(0xffffffffu, target >= 0 && tj >= 0 && tj < 32);
+          if constexpr (EPI == kLse) {
+            if (col0 + 32 > args.N) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                if (col0 + j >= args.N) r[j] = __float_as_uint(-INFINITY);
+            }
+            if (here && target >= 0 && tj >= 0 && tj < 32) {
+              float z = 0.f;
+#pragma unroll
+              for (int j = 0; j < 32; ++j) z = j == tj ? __uint_as_float(r[j]) : z;
+              args.target_logit[row] = z;
+            }
+            float mx = __uint_as_float(r[0]);
+#pragma unroll
+            for (int j = 1; j < 32; ++j) mx = fmaxf(mx, __uint_as_float(r[j]));
+            if (mx > m) {
+              s *= fast_exp2((m - mx) * kLog2e);
+              m = mx;
+            }
+            const float ref = m == -INFINITY ? 0.f : m;  // all -inf so far: the sum stays 0, a NaN shows
+            float s0 = 0.f, s1 = 0.f;
+#pragma unroll
+            for (int j = 0; j < 32; j += 2) {
+              s0 += fast_exp2((__uint_as_float(r[j]) - ref) * kLog2e);
+              s1 += fast_exp2((__uint_as_float(r[j + 1]) - ref) * kLog2e);
+            }
+            s += s0 + s1;
+          } else {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+              // a row without weight is exactly zero, whatever its logits are
+              const float p = fast_exp2(fmaf(__uint_as_float(r[j]) - m, kLog2e, -s));
+              r[j] = __float_as_uint(scale != 0.f ? p * scale : 0.f);
+            }
+            if (here && target >= 0 && tj >= 0 && tj < 32) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j)
+                if (j == tj) r[j] = __float_as_uint(__uint_as_float(r[j]) - scale);
+            }
+            unsigned char* box = boxes + (nbox % kSlots) * kBox;
+            if (lane == 0) asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(kSlots - 1) : "memory");
+            __syncwarp();
+            stage_row<OutT>(box, lane, 1.f, r);
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              tma_store_box(&tmC, box, col0, row0, 0);
+              asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+            }
+            ++nbox;
+          }
+        }
+        if constexpr (EPI == kLse) {
+          if (in) args.part[(int64_t)tn * args.M + row] = make_float2(m, s);
+        }
+        if (tracer) trace_unit(args, kTrEpiEnd, ui);
+        if (++acc == 2) { acc = 0; acc_phase ^= 1; }
+        continue;
+      }
+      const int bo = args.split_c ? unit / num_tiles : bi;  // the matrix of C
 #pragma unroll 1
       for (int c = 0; c < BN / 32; ++c) {
         uint32_t r[32];
@@ -683,12 +797,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           // the store issued from this slot kSlots boxes ago has finished reading it
           if (lane == 0) asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(kSlots - 1) : "memory");
           __syncwarp();
-          stage_row<OutT>(box, lane, args.alpha, r);
+          stage_row<OutT>(box, lane, alpha, r);
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) {
-            if constexpr (EPI == kAccumF32) tma_reduce_add_box(&tmC, box, col0, row0, bi);
-            else tma_store_box(&tmC, box, col0, row0, bi);
+            if constexpr (EPI == kAccumF32) tma_reduce_add_box(&tmC, box, col0, row0, bo);
+            else tma_store_box(&tmC, box, col0, row0, bo);
             asm volatile("cp.async.bulk.commit_group;" ::: "memory");
           }
           ++nbox;
@@ -1072,6 +1186,117 @@ void gemm_pair_rope(const at::Tensor& X, const at::Tensor& W, at::Tensor& Out, c
   PairArgs args{Out.data_ptr(), o.ld, (int)M, (int)N, (int)K, 1.f, 1, 1, 1, GROUP_M, 1, 0,
                 cos_t.data_ptr<float>(), sin_t.data_ptr<float>(), (int)seq, (int)pos0, (int)rot_cols, cos_t.size(1)};
   launch_t<__nv_bfloat16, kRoPE, true, false, false>(ta, tb, tc, args, pairs);
+}
+
+// ------------------------------------------------------------------ linear + cross entropy
+// Operands of the head: h (M, d) and w (N, d), one 16-bit type, K-major.
+static void check_head(const at::Tensor& H, const Mat& h, const at::Tensor& W, const Mat& w) {
+  LRB_CHECK(H.dim() == 2 && W.dim() == 2 && H.scalar_type() == W.scalar_type() && h.cols == w.cols,
+            "linear cross entropy: h (N, d) and w (V, d) of one dtype");
+  LRB_CHECK(tma_ok(H, h) && tma_ok(W, w) && h.cols % 8 == 0,
+            "linear cross entropy: d must be a multiple of 8, rows 16-byte aligned");
+  LRB_CHECK(h.rows < (1LL << 30) && w.rows < (1LL << 30) && h.cols > 0 && h.cols < (1LL << 30),
+            "linear cross entropy: dimensions too large");
+}
+
+// Tile columns of the forward: the first dimension of `part`.
+int64_t gemm_pair_lse_tiles(int64_t V) { return (V + BN - 1) / BN; }
+
+// part (tiles, M) of (max, sum) pairs and the target logits (M) of h w^T (not written
+// where a target is outside [0, V)).
+void gemm_pair_lse(const at::Tensor& H, const at::Tensor& W, const at::Tensor& targets, at::Tensor& part,
+                   at::Tensor& target_logit) {
+  const Mat h = check_operand(H, "h", true), w = check_operand(W, "w", true);
+  check_head(H, h, W, w);
+  const int64_t M = h.rows, N = w.rows, K = h.cols;
+  const bool bf = H.scalar_type() == at::kBFloat16;
+  CUtensorMap ta = make_map(H.data_ptr(), 1, M, K, h.ld, 0, BK, BM, bf);
+  CUtensorMap tb = make_map(W.data_ptr(), 1, N, K, w.ld, 0, BK, BN / 2, bf);
+  const int64_t tiles = ((M + 2 * BM - 1) / (2 * BM)) * ((N + BN - 1) / BN);
+  LRB_CHECK(tiles < (1LL << 30), "linear cross entropy: dimensions too large");
+  const int pairs = (int)std::max<int64_t>(1, std::min<int64_t>(tiles, max_pairs(H.get_device())));
+  PairArgs args{};
+  args.M = (int)M, args.N = (int)N, args.K = (int)K;
+  args.alpha = 1.f, args.splits = 1, args.batch = 1, args.group_m = N >= 16384 ? 16 : GROUP_M;
+  args.targets = targets.data_ptr<int64_t>();
+  args.part = reinterpret_cast<float2*>(part.data_ptr<float>());
+  args.target_logit = target_logit.data_ptr<float>();
+  if (bf) launch_t<__nv_bfloat16, kLse, true, false, false>(ta, tb, ta, args, pairs);
+  else launch_t<__half, kLse, false, false, false>(ta, tb, ta, args, pairs);
+}
+
+// out (M, piece) = (softmax - onehot) * row_scale for the vocabulary rows `W` of the
+// piece that starts at `v0`.
+void gemm_pair_ce_grad(const at::Tensor& H, const at::Tensor& W, const at::Tensor& targets, int64_t v0,
+                       const at::Tensor& stats, const at::Tensor& row_scale, at::Tensor& out) {
+  const Mat h = check_operand(H, "h", true), w = check_operand(W, "w", true), o = check_operand(out, "out", true);
+  check_head(H, h, W, w);
+  const int64_t M = h.rows, N = w.rows, K = h.cols;
+  LRB_CHECK(o.rows == M && o.cols == N && out.scalar_type() == H.scalar_type() && tma_ok(out, o),
+            "linear cross entropy: bad piece buffer");
+  const bool bf = H.scalar_type() == at::kBFloat16;
+  CUtensorMap ta = make_map(H.data_ptr(), 1, M, K, h.ld, 0, BK, BM, bf);
+  CUtensorMap tb = make_map(W.data_ptr(), 1, N, K, w.ld, 0, BK, BN / 2, bf);
+  CUtensorMap tc = make_out_map(out.data_ptr(), 1, M, N, o.ld, 0, out.scalar_type());
+  const int64_t tiles = ((M + 2 * BM - 1) / (2 * BM)) * ((N + BN - 1) / BN);
+  LRB_CHECK(tiles < (1LL << 30), "linear cross entropy: dimensions too large");
+  const int pairs = (int)std::max<int64_t>(1, std::min<int64_t>(tiles, max_pairs(H.get_device())));
+  PairArgs args{};
+  args.M = (int)M, args.N = (int)N, args.K = (int)K;
+  args.alpha = 1.f, args.tma_out = 1, args.splits = 1, args.batch = 1, args.group_m = N >= 16384 ? 16 : GROUP_M;
+  args.targets = targets.data_ptr<int64_t>();
+  args.col0 = v0;
+  args.stats = reinterpret_cast<const float2*>(stats.data_ptr<float>());
+  args.row_scale = row_scale.data_ptr<float>();
+  if (bf) launch_t<__nv_bfloat16, kCeGrad, true, false, false>(ta, tb, tc, args, pairs);
+  else launch_t<__half, kCeGrad, false, false, false>(ta, tb, tc, args, pairs);
+}
+
+// K ranges that let a product of few tiles use every CTA pair: each of at least 8
+// k-blocks, all units in one wave.  1 where the tiles alone fill the pairs.
+int gemm_pair_slices(int64_t M, int64_t N, int64_t K, int dev) {
+  const int64_t tiles = ((M + 2 * BM - 1) / (2 * BM)) * ((N + BN - 1) / BN), nk = (K + BK - 1) / BK;
+  return (int)std::max<int64_t>(1, std::min<int64_t>({max_pairs(dev) / std::max<int64_t>(tiles, 1), nk / 8, 64}));
+}
+
+// C (S, M, N) fp32 (+)= the product over each of `splits` <= S ranges of K, slice by
+// slice (no two of them meet in one element, so nothing depends on their order); or,
+// with a 16-bit 2-D C, C = alpha_dev * A B in one piece.
+void gemm_pair_sliced(const at::Tensor& A, const at::Tensor& B, bool a_mn, bool b_mn, at::Tensor& C, int splits,
+                      bool accumulate, const float* alpha_dev) {
+  const Mat a = check_operand(A, "A", true), b = check_operand(B, "B", true), c = check_operand(C, "C", false);
+  const int64_t M = a_mn ? a.cols : a.rows, K = a_mn ? a.rows : a.cols;
+  const int64_t N = b_mn ? b.cols : b.rows, KB = b_mn ? b.rows : b.cols;
+  const bool sliced = C.dim() == 3;
+  LRB_CHECK(A.dim() == 2 && B.dim() == 2 && A.scalar_type() == B.scalar_type() && K == KB && c.rows == M && c.cols == N &&
+                K > 0 && (sliced ? C.scalar_type() == at::kFloat : C.scalar_type() == A.scalar_type()) &&
+                (sliced || (!accumulate && splits == 1)) && splits >= 1 && splits <= c.batch &&
+                splits <= (K + BK - 1) / BK,
+            "gemm_pair_sliced: shape or dtype mismatch");
+  LRB_CHECK(tma_ok(A, a) && tma_ok(B, b) && tma_ok(C, c), "gemm_pair_sliced: 16-byte aligned bases and pitches");
+  const bool bf = A.scalar_type() == at::kBFloat16;
+  CUtensorMap ta = a_mn ? make_map(A.data_ptr(), 1, K, M, a.ld, 0, 64, BK, bf)
+                        : make_map(A.data_ptr(), 1, M, K, a.ld, 0, BK, BM, bf);
+  CUtensorMap tb = b_mn ? make_map(B.data_ptr(), 1, K, N, b.ld, 0, 64, BK, bf)
+                        : make_map(B.data_ptr(), 1, N, K, b.ld, 0, BK, BN / 2, bf);
+  CUtensorMap tc = make_out_map(C.data_ptr(), c.batch, M, N, c.ld, c.bstride, C.scalar_type());
+  const int64_t tiles = ((M + 2 * BM - 1) / (2 * BM)) * ((N + BN - 1) / BN);
+  LRB_CHECK(tiles * splits < (1LL << 30), "gemm_pair_sliced: dimensions too large");
+  const int pairs = (int)std::max<int64_t>(1, std::min<int64_t>(tiles * splits, max_pairs(A.get_device())));
+  PairArgs args{};
+  args.M = (int)M, args.N = (int)N, args.K = (int)K;
+  args.alpha = 1.f, args.tma_out = 1, args.splits = splits, args.batch = 1, args.group_m = N >= 16384 ? 16 : GROUP_M;
+  args.alpha_dev = alpha_dev;
+  args.split_c = 1;
+  const auto run = [&](auto bf_c) {
+    constexpr bool BF = decltype(bf_c)::value;
+    using T = std::conditional_t<BF, __nv_bfloat16, __half>;
+    if (!sliced) launch_layout<T, kStore, BF>(a_mn, b_mn, ta, tb, tc, args, pairs);
+    else if (accumulate) launch_layout<float, kAccumF32, BF>(a_mn, b_mn, ta, tb, tc, args, pairs);
+    else launch_layout<float, kStore, BF>(a_mn, b_mn, ta, tb, tc, args, pairs);
+  };
+  if (bf) run(std::true_type{});
+  else run(std::false_type{});
 }
 
 // Points the pair GEMM's pipeline trace at `buf` (int64 CUDA, at least

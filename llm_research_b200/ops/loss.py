@@ -17,6 +17,14 @@ parallelism: every rank of the group multiplies the (replicated) hidden states
 by its ``V / tp`` rows of the head weight only, the per-row log-sum-exp and
 target logit are combined over the group, and the gradients come back
 replicated (``dh`` summed over the shards, ``dW`` gathered from them).
+
+:func:`piecewise_linear_cross_entropy` is the head + loss in pieces of the
+*vocabulary*: no logits are kept, or rounded.  :func:`linear_cross_entropy` walks
+over rows, keeps 16-bit logits of a chunk of rows and forms the gradients in the
+forward (three products); the piecewise form needs the products of the backward
+only when a backward comes (one product forward, three backward: the logits are
+formed twice), takes per-row losses and weights, and its working memory is
+``N * piece`` values whatever the vocabulary.
 """
 
 from __future__ import annotations
@@ -130,6 +138,89 @@ def linear_cross_entropy(h: torch.Tensor, w: torch.Tensor, targets: torch.Tensor
     """``cross_entropy(h @ w.T, targets)`` (mean over targets != ignore_index) with the
     logits formed ``chunk`` rows at a time.  ``h (N, d)``, ``w (V, d)``, ``targets (N,)``."""
     return _LinearCEFn.apply(h.reshape(-1, h.shape[-1]), w, targets.reshape(-1), ignore_index, int(chunk))
+
+
+# ------------------------------------------------ linear + CE in pieces of the vocabulary
+_REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
+_PIECE_BYTES = 256 << 20
+
+
+def _vocab_piece(n: int, V: int) -> int:
+    """Vocabulary rows at a time: a 16-bit ``(n, piece)`` buffer of at most about 256 MB
+    (at least 1024 wide), the vocabulary divided evenly into multiples of 256."""
+    most = max(1024, _PIECE_BYTES // (2 * max(n, 1)))
+    pieces = -(-V // most)
+    return (-(-V // pieces) + 255) // 256 * 256
+
+
+class _PiecewiseLinearCEFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, h, w, targets, ignore_index, reduction, piece):
+        rows, stats, out = native().linear_ce_fwd(h, w, targets, ignore_index, reduction)
+        ctx.save_for_backward(h, w, targets, stats, out)
+        ctx.ignore_index, ctx.reduction, ctx.piece = ignore_index, reduction, piece
+        return rows if reduction == 0 else out[0]
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        h, w, targets, stats, out = ctx.saved_tensors
+        per_row = ctx.reduction == 0
+        need_h, need_w = ctx.needs_input_grad[:2]
+        dh, dw = native().linear_ce_bwd(h, w, targets, ctx.ignore_index, stats, g.float().contiguous(), per_row,
+                                        stats if per_row else out[1:], ctx.piece, need_h, need_w)
+        return dh if need_h else None, dw if need_w else None, None, None, None, None
+
+
+def piecewise_linear_cross_entropy(h: torch.Tensor, w: torch.Tensor, targets: torch.Tensor, ignore_index: int = -100,
+                                   reduction: str = "mean", piece: int | None = None) -> torch.Tensor:
+    """``cross_entropy(h @ w.T, targets)`` without keeping the logits.
+
+    ``h (..., d)``, ``w (V, d)``, ``targets`` int64 of ``h``'s leading shape.  A row
+    counts unless its target is ``ignore_index`` or outside ``[0, V)``; ``reduction``
+    is ``"mean"`` over the counted rows (0 without any), ``"sum"`` or ``"none"`` (the
+    leading shape, 0 in rows that do not count), fp32.  CUDA: bf16 or fp16, ``d`` a
+    multiple of 8, on the CTA-pair tensor-core kernel (``csrc/kernels/linear_ce.cu``):
+    the log-sum-exp is taken from the fp32 products, and the backward forms the
+    logits' gradient for ``piece`` vocabulary rows at a time (default: a buffer of
+    about 256 MB).  As in any matrix product, an ``inf`` or NaN in a row of ``h``
+    that does not count still reaches ``dw`` (0 * inf)."""
+    if reduction not in _REDUCTIONS:
+        raise ValueError(f"piecewise_linear_cross_entropy: reduction must be one of {sorted(_REDUCTIONS)}, "
+                         f"got {reduction!r}")
+    if w.dim() != 2 or h.dim() < 1 or h.shape[-1] != w.shape[1] or targets.shape != h.shape[:-1] or w.shape[0] < 1:
+        raise ValueError(f"piecewise_linear_cross_entropy: h (..., d), w (V, d), targets (...), got "
+                         f"{tuple(h.shape)}, {tuple(w.shape)}, {tuple(targets.shape)}")
+    if targets.dtype != torch.int64:
+        raise TypeError(f"piecewise_linear_cross_entropy: targets must be int64, got {targets.dtype}")
+    if piece is not None and piece < 1:
+        raise ValueError(f"piecewise_linear_cross_entropy: piece must be positive, got {piece}")
+    V, d = w.shape
+    lead, rows = targets.shape, targets.numel()
+    h2, t = h.reshape(rows, d), targets.reshape(rows)
+    if not h.is_cuda:
+        f = torch.float64 if h.dtype == torch.float64 else torch.float32
+        counted = (t != ignore_index) & (t >= 0) & (t < V)
+        logq = torch.log_softmax(F.linear(h2.to(f), w.to(f)), dim=-1)
+        loss = -logq.gather(1, t.clamp(0, V - 1)[:, None]).squeeze(1)
+        loss = torch.where(counted, loss, torch.zeros_like(loss))
+        if reduction == "none":
+            return loss.reshape(lead)
+        return loss.sum() if reduction == "sum" else loss.sum() / counted.sum().clamp(min=1)
+    if h.dtype not in (torch.bfloat16, torch.float16) or w.dtype != h.dtype:
+        raise TypeError(f"piecewise_linear_cross_entropy: h and w must both be bf16 or both fp16 on CUDA, got "
+                        f"{h.dtype} and {w.dtype} (linear_cross_entropy takes other types)")
+    if d % 8:
+        raise ValueError(f"piecewise_linear_cross_entropy: d must be a multiple of 8 on CUDA, got {d}")
+    piece = _vocab_piece(rows, V) if piece is None else (int(piece) + 7) // 8 * 8
+    h2, w = _rows(h2), _rows(w)
+    code = _REDUCTIONS[reduction]
+    if torch.is_grad_enabled() and (h2.requires_grad or w.requires_grad):
+        loss = _PiecewiseLinearCEFn.apply(h2, w, t.contiguous(), int(ignore_index), code, piece)
+    else:
+        losses, _, out = native().linear_ce_fwd(h2, w, t.contiguous(), int(ignore_index), code)
+        loss = losses if code == 0 else out[0]
+    return loss.view(lead) if code == 0 else loss
 
 
 # ------------------------------------------------ vocabulary-parallel linear + CE
