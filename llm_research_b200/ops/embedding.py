@@ -5,9 +5,8 @@
 sums in fp32, one rounding to the weight's dtype (bf16, fp16 or fp32).
 
 CUDA (``csrc/kernels/embedding.cu``): the lookup is one kernel; the gradient
-sorts the tokens (one cluster, stable) and writes every row of ``dW`` once, the
-occurrences of a token added in the order of their positions: the same inputs
-give the same bits.  ``padding_idx`` only leaves its row out of the gradient
+sorts the tokens (one cluster, stable) and adds the occurrences of a token in the
+order of their positions: the same inputs give the same bits.  ``padding_idx`` only leaves its row out of the gradient
 (``F.embedding`` semantics).  An id outside ``[0, V)`` cannot be reported from
 the device without a synchronisation: its output row is NaN and it has no
 gradient (on the CPU it raises ``IndexError``).
@@ -35,7 +34,13 @@ class _EmbeddingFn(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dy):
         ids, = ctx.saved_tensors
-        return _EmbeddingGradFn.apply(dy, ids, ctx.rows, ctx.scale, ctx.padding), None, None, None
+        if torch.is_grad_enabled():  # create_graph
+            return _EmbeddingGradFn.apply(dy, ids, ctx.rows, ctx.scale, ctx.padding), None, None, None
+        return _grad(dy, ids, ctx.rows, ctx.scale, ctx.padding), None, None, None
+
+
+def _grad(dy, ids, rows, scale, padding):
+    return native().embedding_bwd(dy if dy.stride(-1) == 1 else dy.contiguous(), ids, rows, padding, scale)
 
 
 class _EmbeddingGradFn(torch.autograd.Function):
@@ -46,9 +51,7 @@ class _EmbeddingGradFn(torch.autograd.Function):
     def forward(ctx, dy, ids, rows, scale, padding):
         ctx.save_for_backward(ids)
         ctx.rows, ctx.scale, ctx.padding = rows, scale, padding
-        if dy.stride(-1) != 1:
-            dy = dy.contiguous()
-        return native().embedding_bwd(dy, ids, rows, padding, scale)
+        return _grad(dy, ids, rows, scale, padding)
 
     @staticmethod
     def backward(ctx, g):
