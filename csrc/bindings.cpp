@@ -34,8 +34,8 @@ std::tuple<at::Tensor, at::Tensor> linear_ce_bwd(const at::Tensor&, const at::Te
                                                  bool, bool);
 // distill.cu
 std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> distill_fwd(const at::Tensor&, const at::Tensor&,
-                                                                       const at::Tensor&, double, int64_t);
-at::Tensor distill_bwd(const at::Tensor&, const at::Tensor&, const at::Tensor&, double, const at::Tensor&,
+                                                                       const at::Tensor&, double, int64_t, bool);
+at::Tensor distill_bwd(const at::Tensor&, const at::Tensor&, double, const at::Tensor&, const at::Tensor&,
                        const at::Tensor&, bool, const at::Tensor&);
 // routing.cu
 std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> route_slots(const at::Tensor&, int64_t, int64_t, int64_t);

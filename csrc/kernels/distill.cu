@@ -8,13 +8,17 @@
 //   loss_n  = T^2 sum_k p_k (ln p_k - ln q[id_k])
 //   dx_j    = T g_n (q_j - sum of p_k with id_k = j)
 //
-// The vocabulary is read once per direction: the forward keeps a running maximum
-// m and a running sum s of exp((x - m) / T) per thread and joins them; (m, log2 s)
-// of each row is all that the backward needs.  All of it is fp32.  Differences
-// x - m are formed before the scaling by log2(e) / T, so that a row of the type's
-// lowest values does not overflow.
+// The vocabulary is read once per direction.  The forward keeps a running maximum and
+// a running sum per thread and joins them; the backward needs four numbers a row and
+// the probabilities p.  Everything is fp32, in powers of two with k2 = log2(e) / T:
+// with B = m k2 rounded once (any reference near the maximum would do, as long as both
+// sides use the same), log2 q_j = (x_j k2 - B) - log2 s, the bracket one fma.
+// Rows whose maximum is beyond 1e30, where x k2 - B would overflow (a row of the
+// type's lowest values), take differences x - m first.
 //
-// Bounded by the bytes of the logits.
+// Bounded by the bytes of the logits; for 16-bit logits the 16 exponentials a clock
+// and SM are the next limit (12 at the copy rate), so the rest is kept short: maxima
+// of 16-bit pairs, packed fp32 fma and add.
 #include "../common.cuh"
 
 #include <cmath>
@@ -22,10 +26,21 @@
 namespace lrb {
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kMaxK = 1024;                    // teacher entries of a row
-constexpr int kPerThread = kMaxK / kThreads;   // held in registers
+constexpr int kThreads = 256, kWarps = kThreads / 32;
+constexpr int kPerThread = 4;                   // teacher entries a thread holds
+constexpr int kMaxK = kPerThread * kThreads;    // entries of a row, for a block a row
+constexpr int kWarpK = kPerThread * 32;         // for a warp a row
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kFar = 1e30f;
+
+// Vectors in flight a thread (U) and blocks an SM, measured: 16384 x 32000 bf16 forward
+// 199 us at 8 / 4 with a warp a row and 201 to 218 us at 4 / 5 and 4 / 6 with a block a row;
+// 4093 x 100287 fp32 261 us at 8 / 4 (291 at 4 / 6).  Backward 320 us at 4 / 5 (335 at
+// 4 / 8, 338 at 8 / 4) and 559 us at 4 / any (587 at 4 / 5).
+template <typename T, int W> constexpr int kFwdU = W == 1 || sizeof(T) == 4 ? 8 : 4;
+template <typename T, int W> constexpr int kFwdBlocks = W == 1 || sizeof(T) == 4 ? 4 : 5;
+template <typename T, int W> constexpr int kBwdU = W == 1 ? 8 : 4;
+template <typename T, int W> constexpr int kBwdBlocks = W == 1 ? 4 : sizeof(T) == 4 ? 1 : 5;
 
 struct Teacher {
   const void* logits;  // (N, K) bf16 / fp16 / fp32
@@ -45,69 +60,122 @@ __device__ __forceinline__ int teacher_id(const Teacher& t, int64_t i, int V) { 
   return id >= 0 && id < V ? (int)id : -1;
 }
 
-// This thread's entries k = threadIdx.x + i * kThreads: token (-1: none) and
-// probability; returns whether the row has any.  ln p_k = y_k / T - ln(sum), left in `lp`.
-__device__ __forceinline__ bool teacher_probs(const Teacher& t, int64_t row, int V, float inv_t, float* red,
-                                              int (&id)[kPerThread], float (&p)[kPerThread], float (&lp)[kPerThread]) {
-  float mx = -INFINITY;
-  int any = 0;
-#pragma unroll
-  for (int i = 0; i < kPerThread; ++i) {
-    const int k = threadIdx.x + i * kThreads;
-    id[i] = -1;
-    lp[i] = -INFINITY;
-    if (k < t.K) {
-      const int v = teacher_id(t, row * t.K + k, V);
-      if (v >= 0) {
-        const float y = teacher_logit(t, row * t.K + k);
-        if (y != -INFINITY) {
-          id[i] = v;
-          lp[i] = y;
-          mx = fmaxf(mx, y);
-          any = 1;
-        }
-      }
-    }
-  }
-  if (!__syncthreads_or(any)) return false;
-  mx = block_max(mx, red);
-  float sum = 0.f;
-#pragma unroll
-  for (int i = 0; i < kPerThread; ++i) {
-    lp[i] = (lp[i] - mx) * inv_t;
-    p[i] = id[i] >= 0 ? expf(lp[i]) : 0.f;
-    sum += p[i];
-  }
-  sum = block_sum(sum, red);
-  const float inv = 1.f / sum, ls = logf(sum);
-#pragma unroll
-  for (int i = 0; i < kPerThread; ++i) {
-    p[i] *= inv;
-    lp[i] -= ls;
-  }
-  return true;
-}
+// What the forward leaves for the backward.
+struct RowStats {
+  float base, log2_s, m, counted;
+};
 
-// Running (max, sum of 2^((x - max) k2)).  A maximum of -inf (nothing but -inf so
-// far) uses 0 as its reference: 2^-inf = 0, and a NaN still reaches the sum.
-struct Online {
-  float m = -INFINITY, s = 0.f;
-  __device__ __forceinline__ void raise(float mx, float k2) {
-    if (mx > m) {
-      s *= fast_exp2((m - mx) * k2);
-      m = mx;
-    }
+template <typename T> struct Pairs;  // a 16-byte vector as packed fp32 pairs, and its maximum
+template <> struct Pairs<__nv_bfloat16> {
+  static constexpr int N = 4;
+  static __device__ __forceinline__ uint64_t get(const uint4& r, int i) {
+    const uint32_t w = i == 0 ? r.x : i == 1 ? r.y : i == 2 ? r.z : r.w;
+    return f2_pack(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
   }
-  __device__ __forceinline__ float ref() const { return m == -INFINITY ? 0.f : m; }
-  __device__ __forceinline__ void add(float x, float k2) {
-    raise(x, k2);
-    s += fast_exp2((x - ref()) * k2);
+  static __device__ __forceinline__ uint32_t put(float2 v) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(v.x, v.y);
+    return *reinterpret_cast<const uint32_t*>(&h);
   }
-  __device__ __forceinline__ void merge(float m2, float s2, float k2) {
-    raise(m2, k2);
-    s += s2 * fast_exp2((m2 - ref()) * k2);  // m2 = -inf: s2 is 0 or NaN, times 0
+  template <int U>
+  static __device__ __forceinline__ float max(const uint4 (&r)[U]) {
+    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&r);
+    __nv_bfloat162 m = h[0];
+#pragma unroll
+    for (int i = 1; i < 4 * U; ++i) m = __hmax2(m, h[i]);
+    const float2 f = __bfloat1622float2(m);
+    return fmaxf(f.x, f.y);
   }
 };
+template <> struct Pairs<__half> {
+  static constexpr int N = 4;
+  static __device__ __forceinline__ uint64_t get(const uint4& r, int i) {
+    const uint32_t w = i == 0 ? r.x : i == 1 ? r.y : i == 2 ? r.z : r.w;
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+    return f2_pack(f.x, f.y);
+  }
+  static __device__ __forceinline__ uint32_t put(float2 v) {
+    const __half2 h = __floats2half2_rn(v.x, v.y);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+  template <int U>
+  static __device__ __forceinline__ float max(const uint4 (&r)[U]) {
+    const __half2* h = reinterpret_cast<const __half2*>(&r);
+    __half2 m = h[0];
+#pragma unroll
+    for (int i = 1; i < 4 * U; ++i) m = __hmax2(m, h[i]);
+    const float2 f = __half22float2(m);
+    return fmaxf(f.x, f.y);
+  }
+};
+template <> struct Pairs<float> {
+  static constexpr int N = 2;
+  static __device__ __forceinline__ uint64_t get(const uint4& r, int i) {
+    return i == 0 ? f2_pack(__uint_as_float(r.x), __uint_as_float(r.y))
+                  : f2_pack(__uint_as_float(r.z), __uint_as_float(r.w));
+  }
+  template <int U>
+  static __device__ __forceinline__ float max(const uint4 (&r)[U]) {
+    const float* f = reinterpret_cast<const float*>(&r);
+    float m = f[0];
+#pragma unroll
+    for (int i = 1; i < 4 * U; ++i) m = fmaxf(m, f[i]);
+    return m;
+  }
+};
+
+// The base that goes with a maximum.  Rounded here: contracted into a following
+// subtraction, the bases of one maximum would differ by their rounding (1e22 at 1e30).
+__device__ __forceinline__ float base_of(float m, float k2) { return __fmul_rn(fminf(fmaxf(m, -kFar), kFar), k2); }
+
+// Running maximum m and sum of 2^(x k2 - base), base = ref k2 with ref the maximum kept
+// within +-1e30: below, everything so far adds nothing (2^-huge = 0), and a NaN shows.
+struct Online {
+  float m = -INFINITY, base;
+  uint64_t s = 0;  // two partial sums
+  __device__ __forceinline__ explicit Online(float k2) : base(base_of(-INFINITY, k2)) {}
+  __device__ __forceinline__ void raise(float mx, float k2) {
+    if (mx > m) {
+      const float b = base_of(mx, k2);
+      const float f = fast_exp2(base - b);
+      s = f2_mul(s, f2_pack(f, f));
+      m = mx;
+      base = b;
+    }
+  }
+  __device__ __forceinline__ void add(float x, float k2) {
+    raise(x, k2);
+    s = f2_add(s, f2_pack(fast_exp2(fmaf(x, k2, -base)), 0.f));
+  }
+  template <typename T, int U>
+  __device__ __forceinline__ void add_vecs(const uint4 (&r)[U], float k2) {
+    raise(Pairs<T>::template max<U>(r), k2);  // one for all of them
+    const uint64_t kk = f2_pack(k2, k2), nb = f2_pack(-base, -base);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < Pairs<T>::N; ++i) {
+        const float2 e = f2_unpack(f2_fma(Pairs<T>::get(r[u], i), kk, nb));
+        s = f2_add(s, f2_pack(fast_exp2(e.x), fast_exp2(e.y)));
+      }
+  }
+  __device__ __forceinline__ float sum() const {
+    const float2 v = f2_unpack(s);
+    return v.x + v.y;
+  }
+};
+
+// (m, s) pairs whose s refer to the base of their own m.
+__device__ __forceinline__ float2 join(float2 a, float2 b, float k2) {
+  const float m = fmaxf(a.x, b.x);
+  const float base = base_of(m, k2);
+  return make_float2(m, a.y * fast_exp2(base_of(a.x, k2) - base) + b.y * fast_exp2(base_of(b.x, k2) - base));
+}
+__device__ __forceinline__ float2 warp_join(float2 v, float k2) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+    v = join(v, make_float2(__shfl_xor_sync(0xffffffffu, v.x, o), __shfl_xor_sync(0xffffffffu, v.y, o)), k2);
+  return v;
+}
 
 __device__ __forceinline__ unsigned cluster_rank() {
   unsigned r;
@@ -141,100 +209,182 @@ __device__ __forceinline__ const T* row_ptr(const T* x, const Rows& r, int64_t n
   return x + o * r.s_outer + (n - o * r.inner) * r.s_inner;
 }
 
-// One cluster per row; its blocks take equal ranges of the vocabulary (more than
-// one block only where there are too few rows to fill the GPU).
-template <typename T>
-__global__ void __launch_bounds__(kThreads)
-    distill_fwd_kernel(const T* __restrict__ logits, Rows rows, int V, Teacher t, float temp, float* __restrict__ loss,
-                       float* __restrict__ counted, float2* __restrict__ stats) {
-  __shared__ float red[32];
-  __shared__ float2 part[kThreads / 32], mine;
-  constexpr int VEC = 16 / sizeof(T), U = 4;
-  const unsigned rank = cluster_rank(), split = cluster_size();
-  const int64_t row = blockIdx.x / split;
+// The elements of [p, p + len) by `step` threads: `one` for those before the first and
+// behind the last 16-byte boundary, `all` for U vectors at a time (loaded together, no
+// bounds to look at), `vec` for the last ones.
+template <int U, typename T, typename One, typename All, typename Vec>
+__device__ __forceinline__ void walk(const T* p, int len, int tid, int step, One one, All all, Vec vec) {
+  constexpr int VEC = 16 / sizeof(T);
+  const int head = min(len, (int)(((16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15) / sizeof(T)));
+  const int nvec = (len - head) / VEC, tail = len - head - nvec * VEC;
+  if (tid < head) one(tid);
+  if (tid < tail) one(len - tail + tid);
+  const uint4* b = reinterpret_cast<const uint4*>(p + head);
+  int i = tid;
+  for (; i + (U - 1) * step < nvec; i += U * step) {
+    uint4 v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) v[u] = __ldg(b + i + u * step);
+    all(head + i * VEC, step * VEC, v);
+  }
+  if (i < nvec) {
+    uint4 v[U - 1];
+#pragma unroll
+    for (int u = 0; u < U - 1; ++u)
+      if (i + u * step < nvec) v[u] = __ldg(b + i + u * step);
+#pragma unroll
+    for (int u = 0; u < U - 1; ++u)
+      if (i + u * step < nvec) vec(head + (i + u * step) * VEC, v[u]);
+  }
+}
+
+// The teacher's side of a row over some of its entries, w = 2^((y - mx) k2):
+// S0 = sum w, S1 = sum w (y - mx) k2, S2 = sum w (x[id] - ref) k2, so that
+// sum p (log2 p - (x[id] - ref) k2) = (S1 - S2) / S0 - log2 S0.  S0 = 0: no entries.
+struct Entries {
+  float mx, s0, s1, s2;
+};
+__device__ __forceinline__ Entries join(const Entries& a, const Entries& b, float k2) {
+  const float mx = fmaxf(a.mx, b.mx);
+  Entries r{mx, 0.f, 0.f, 0.f};
+  const auto put = [&](const Entries& e) {
+    if (e.s0 == 0.f) return;
+    const float d = e.mx == mx ? 0.f : (e.mx - mx) * k2, f = fast_exp2(d);
+    if (f == 0.f && e.s0 == e.s0) return;
+    r.s0 += f * e.s0;
+    r.s1 += f * (e.s1 + e.s0 * d);
+    r.s2 += f * e.s2;
+  };
+  put(a);
+  put(b);
+  return r;
+}
+
+// W = 1: a row a warp, without any barrier.  W = 8: a row a block, or, where the rows
+// do not fill the GPU, a cluster whose blocks take equal ranges of the vocabulary (the
+// first one does the teacher's side).
+template <typename T, int W>
+__global__ void __launch_bounds__(kThreads, (kFwdBlocks<T, W>))
+    distill_fwd_kernel(const T* __restrict__ logits, Rows rows, int64_t n, int V, Teacher t, float temp,
+                       float* __restrict__ loss, float* __restrict__ counted, RowStats* __restrict__ stats,
+                       float* __restrict__ probs) {
+  __shared__ float2 part[kWarps], mine;
+  __shared__ Entries entries[kWarps];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const unsigned rank = W == 1 ? 0 : cluster_rank(), split = W == 1 ? 1 : cluster_size();
+  const int64_t row = W == 1 ? (int64_t)blockIdx.x * kWarps + warp : blockIdx.x / split;
+  if (row >= n) return;  // W = 1 only: whole warps
   const T* x = row_ptr(logits, rows, row);
   const int c0 = (int)((int64_t)V * rank / split), c1 = (int)((int64_t)V * (rank + 1) / split);
-  const float inv_t = 1.f / temp, k2 = kLog2e * inv_t;
+  const float k2 = kLog2e / temp;
+  const int tid = W == 1 ? lane : threadIdx.x;
 
-  Online a;
-  {
-    const T* p = x + c0;
-    const int len = c1 - c0;
-    const int head = min(len, (int)(((16 - (reinterpret_cast<uintptr_t>(p) & 15)) & 15) / sizeof(T)));
-    const int nvec = (len - head) / VEC, tail = len - head - nvec * VEC;
-    if (threadIdx.x < head) a.add(to_f(p[threadIdx.x]), k2);
-    if (threadIdx.x < tail) a.add(to_f(p[len - tail + threadIdx.x]), k2);
-    const T* b = p + head;
-    for (int i = threadIdx.x; i < nvec; i += U * kThreads) {
-      Vec16<T> v[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (i + u * kThreads < nvec) v[u] = ld16(b + (int64_t)(i + u * kThreads) * VEC);
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (i + u * kThreads >= nvec) break;
-        float f[VEC], mx = -INFINITY;
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) {
-          f[j] = to_f(v[u].v[j]);
-          mx = fmaxf(mx, f[j]);
-        }
-        a.raise(mx, k2);
-        const float r = a.ref();
-        float s = 0.f;
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) s += fast_exp2((f[j] - r) * k2);
-        a.s += s;
-      }
-    }
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const float m2 = __shfl_xor_sync(0xffffffffu, a.m, o), s2 = __shfl_xor_sync(0xffffffffu, a.s, o);
-    a.merge(m2, s2, k2);
-  }
-  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = make_float2(a.m, a.s);
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    Online b;
-    for (int w = 0; w < kThreads / 32; ++w) b.merge(part[w].x, part[w].y, k2);
-    mine = make_float2(b.m, b.s);
-  }
-  if (split > 1) {
-    cluster_barrier();
-    if (rank == 0 && threadIdx.x == 0) {
-      Online b;
-      for (unsigned r = 0; r < split; ++r) {
-        const float2 o = ld_peer(&mine, r);
-        b.merge(o.x, o.y, k2);
-      }
-      part[0] = make_float2(b.m, b.s);
-    }
-    cluster_barrier();  // every block's `mine` has been read
-    if (rank != 0) return;
-  } else {
-    __syncthreads();
-    if (threadIdx.x == 0) part[0] = mine;
-  }
-  __syncthreads();
-  const float m = part[0].x, s = part[0].y;
-  const float log2_s = log2f(s);
-  if (threadIdx.x == 0) stats[row] = make_float2(m, log2_s);
-
+  // The first entry of each thread (mostly the only one) is loaded ahead of the long walk
+  // and looked at behind it.
   int id[kPerThread];
-  float p[kPerThread], lp[kPerThread];
-  const bool some = teacher_probs(t, row, V, inv_t, red, id, p, lp);
-  float acc = 0.f;
-  if (some) {
-    const float ls = log2_s * kLn2;
+  float y[kPerThread];
+  const auto load_entry = [&](int i) {
+    const int k = tid + i * 32 * W;
+    id[i] = -1;
+    y[i] = 0.f;
+    if (k < t.K) {
+      id[i] = teacher_id(t, row * t.K + k, V);
+      y[i] = teacher_logit(t, row * t.K + k);
+    }
+  };
+  if (rank == 0) load_entry(0);
+  Online o(k2);
+  constexpr int U = kFwdU<T, W>;
+  walk<U>(
+      x + c0, c1 - c0, tid, 32 * W, [&](int i) { o.add(to_f(x[c0 + i]), k2); },
+      [&](int, int, const uint4 (&v)[U]) { o.add_vecs<T, U>(v, k2); },
+      [&](int, const uint4& v) {
+        const uint4 one[1] = {v};
+        o.add_vecs<T, 1>(one, k2);
+      });
+  float2 ms = warp_join(make_float2(o.m, o.sum()), k2);
+
+  Entries e{-INFINITY, 0.f, 0.f, 0.f};
+  // one of the row's logits: a common offset of all of them loses nothing
+  float ref = 0.f;
+  if (rank == 0 && (W == 1 || warp * 32 < t.K)) {
+    ref = to_f(x[0]);
+    if (!(fabsf(ref) <= kFar)) ref = 0.f;
 #pragma unroll
-    for (int i = 0; i < kPerThread; ++i)
-      if (id[i] >= 0 && p[i] != 0.f) acc += p[i] * (lp[i] - ((to_f(x[id[i]]) - m) * inv_t - ls));
-    acc = block_sum(acc, red);
+    for (int i = 1; i < kPerThread; ++i) load_entry(i);
+    float xg[kPerThread];
+#pragma unroll
+    for (int i = 0; i < kPerThread; ++i) {
+      if (y[i] == -INFINITY) id[i] = -1;
+      xg[i] = id[i] >= 0 ? to_f(x[id[i]]) : 0.f;
+      if (id[i] >= 0) e.mx = fmaxf(e.mx, y[i]);
+    }
+    e.mx = warp_max(e.mx);
+#pragma unroll
+    for (int i = 0; i < kPerThread; ++i) {
+      if (id[i] < 0) continue;
+      const float d = (y[i] - e.mx) * k2, w = fast_exp2(d);
+      if (w == 0.f) continue;
+      e.s0 += w;
+      e.s1 += w * d;
+      e.s2 += w * ((xg[i] - ref) * k2);
+    }
+    e.s0 = warp_sum(e.s0);
+    e.s1 = warp_sum(e.s1);
+    e.s2 = warp_sum(e.s2);
   }
-  if (threadIdx.x == 0) {
-    loss[row] = some ? temp * temp * acc : 0.f;
+  if constexpr (W > 1) {
+    if (lane == 0) {
+      part[warp] = ms;
+      entries[warp] = e;
+    }
+    __syncthreads();
+    if (warp == 0) ms = warp_join(lane < kWarps ? part[lane] : make_float2(-INFINITY, 0.f), k2);
+    if (split > 1) {
+      if (threadIdx.x == 0) mine = ms;
+      cluster_barrier();
+      if (rank == 0 && warp == 0)
+        ms = warp_join(lane < split ? ld_peer(&mine, (unsigned)lane) : make_float2(-INFINITY, 0.f), k2);
+      cluster_barrier();  // every block's `mine` has been read
+      if (rank != 0) return;
+    }
+    e = entries[0];  // every thread joins them, in one order
+#pragma unroll
+    for (int w = 1; w < kWarps; ++w) e = join(e, entries[w], k2);
+  }
+  const bool some = e.s0 != 0.f;
+  if (probs != nullptr) {
+    const float inv = 1.f / e.s0;
+#pragma unroll
+    for (int i = 0; i < kPerThread; ++i) {
+      const int k = tid + i * 32 * W;
+      if (k < t.K) probs[row * t.K + k] = id[i] >= 0 ? fast_exp2((y[i] - e.mx) * k2) * inv : 0.f;
+    }
+  }
+  if (W > 1 && warp != 0) return;
+  const float m = ms.x;
+  float a = (e.s1 - e.s2) / e.s0 - log2f(e.s0);
+  float rest = fmaf(-ref, k2, base_of(m, k2));
+  if (fabsf(m) > kFar && fabsf(m) < INFINITY) {  // differences to m first (this warp alone, the whole row)
+    float s = 0.f;
+    for (int i = lane; i < V; i += 32) s += fast_exp2((to_f(x[i]) - m) * k2);
+    ms.y = warp_sum(s);
+    a = 0.f;
+    for (int k = lane; k < t.K; k += 32) {
+      const int v = teacher_id(t, row * t.K + k, V);
+      const float yk = teacher_logit(t, row * t.K + k);
+      if (v < 0 || yk == -INFINITY) continue;
+      const float lp = (yk - e.mx) * k2 - log2f(e.s0), pk = fast_exp2(lp);
+      if (pk != 0.f) a += pk * (lp - (to_f(x[v]) - m) * k2);
+    }
+    a = warp_sum(a);
+    rest = 0.f;
+  }
+  if (lane == 0) {
+    const float log2_s = log2f(ms.y);
+    stats[row] = RowStats{base_of(m, k2), log2_s, m, some ? 1.f : 0.f};
+    // sum p (log2 p - log2 q) = sum p (log2 p - (x[id] - ref) k2) + (base - ref k2) + log2 s
+    loss[row] = some ? temp * temp * kLn2 * (a + (rest + log2_s)) : 0.f;
     counted[row] = some ? 1.f : 0.f;
   }
 }
@@ -272,106 +422,136 @@ __global__ void __launch_bounds__(1024) reduce_rows_kernel(const float* __restri
   }
 }
 
-// gridDim.x = blocks per row * rows.  Each block writes its range of q scaled, then
-// puts the entries that lie in the range right.
-template <typename T>
-__global__ void __launch_bounds__(kThreads)
-    distill_bwd_kernel(const T* __restrict__ logits, Rows rows, int V, Teacher t, float temp,
-                       const float2* __restrict__ stats, const float* __restrict__ g, int g_per_row,
-                       const float* __restrict__ factor, T* __restrict__ dx, int split) {
-  __shared__ float red[32];
-  __shared__ int ids[kMaxK], seen[2 * kMaxK];
-  __shared__ float probs[kMaxK];
-  constexpr int VEC = 16 / sizeof(T), U = 4;
-  const int64_t row = blockIdx.x / split;
-  const int part = (int)(blockIdx.x - row * split);
+// W = 1: a row a warp; W = 8: `split` blocks a row, each a range of it.  The range of q
+// is written scaled, then the entries that lie in it are put right.  The last rows come
+// first: they are the ones that the forward left in L2.
+template <typename T, int W>
+__global__ void __launch_bounds__(kThreads, (kBwdBlocks<T, W>))
+    distill_bwd_kernel(const T* __restrict__ logits, Rows rows, int64_t n, int V, Teacher t, float temp,
+                       const float* __restrict__ probs, const RowStats* __restrict__ stats, const float* __restrict__ g,
+                       int g_per_row, const float* __restrict__ factor, T* __restrict__ dx, int split) {
+  __shared__ int all_ids[kMaxK], all_seen[2 * kMaxK];
+  __shared__ float all_p[kMaxK];
+  constexpr int VEC = 16 / sizeof(T), G = 32 * W;
+  const int tid = W == 1 ? threadIdx.x & 31 : threadIdx.x, group = W == 1 ? threadIdx.x >> 5 : 0;
+  int* ids = all_ids + group * kWarpK;
+  int* seen = all_seen + group * 2 * kWarpK;
+  float* sp = all_p + group * kWarpK;
+  const unsigned block = gridDim.x - 1 - blockIdx.x;
+  const int64_t row = W == 1 ? (int64_t)block * kWarps + group : block / split;
+  if (row >= n) return;  // W = 1 only: whole warps
+  const int part = W == 1 ? 0 : (int)(block - row * split);
   const T* x = row_ptr(logits, rows, row);
   T* d = dx + row * V;
   const int c0 = (int)((int64_t)V * part / split), c1 = (int)((int64_t)V * (part + 1) / split);
   const int len = c1 - c0;
-  const float inv_t = 1.f / temp, k2 = kLog2e * inv_t;
-
-  int id[kPerThread];
-  float p[kPerThread], lp[kPerThread];
-  const bool some = teacher_probs(t, row, V, inv_t, red, id, p, lp);
-  const T* xp = x + c0;
+  const float4 st = __ldg(reinterpret_cast<const float4*>(stats + row));
+  const float base = st.x, l2 = st.y, m = st.z;
   T* dp = d + c0;
-  if (!some) {
+  if (st.w == 0.f) {  // no teacher
     const int head = min(len, (int)(((16 - (reinterpret_cast<uintptr_t>(dp) & 15)) & 15) / sizeof(T)));
     const int nvec = (len - head) / VEC, tail = len - head - nvec * VEC;
-    if (threadIdx.x < head) dp[threadIdx.x] = from_f<T>(0.f);
-    if (threadIdx.x < tail) dp[len - tail + threadIdx.x] = from_f<T>(0.f);
-    for (int i = threadIdx.x; i < nvec; i += kThreads)
+    if (tid < head) dp[tid] = from_f<T>(0.f);
+    if (tid < tail) dp[len - tail + tid] = from_f<T>(0.f);
+    for (int i = tid; i < nvec; i += G)
       *reinterpret_cast<uint4*>(dp + head + (int64_t)i * VEC) = make_uint4(0u, 0u, 0u, 0u);
     return;
   }
+  const float k2 = kLog2e / temp;
   const float coef = temp * (g_per_row ? g[row] : g[0] * factor[0]);
-  const float m = stats[row].x, l2 = stats[row].y;
-  const auto q = [&](float v) { return fast_exp2((v - m) * k2 - l2); };
-  if ((reinterpret_cast<uintptr_t>(xp) & 15) == (reinterpret_cast<uintptr_t>(dp) & 15)) {
-    const int head = min(len, (int)(((16 - (reinterpret_cast<uintptr_t>(dp) & 15)) & 15) / sizeof(T)));
-    const int nvec = (len - head) / VEC, tail = len - head - nvec * VEC;
-    if (threadIdx.x < head) dp[threadIdx.x] = from_f<T>(coef * q(to_f(xp[threadIdx.x])));
-    if (threadIdx.x < tail) dp[len - tail + threadIdx.x] = from_f<T>(coef * q(to_f(xp[len - tail + threadIdx.x])));
-    const T* b = xp + head;
-    T* o = dp + head;
-    for (int i = threadIdx.x; i < nvec; i += U * kThreads) {
-      Vec16<T> v[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (i + u * kThreads < nvec) v[u] = ld16(b + (int64_t)(i + u * kThreads) * VEC);
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        if (i + u * kThreads >= nvec) break;
-#pragma unroll
-        for (int j = 0; j < VEC; ++j) v[u].v[j] = from_f<T>(coef * q(to_f(v[u].v[j])));
-        st16(o + (int64_t)(i + u * kThreads) * VEC, v[u]);
-      }
-    }
-  } else {
-    for (int i = threadIdx.x; i < len; i += kThreads) dp[i] = from_f<T>(coef * q(to_f(xp[i])));
-  }
+  const bool far = !(fabsf(m) <= kFar);
+  const auto q = [&](float v) { return fast_exp2((far ? (v - m) * k2 : fmaf(v, k2, -base)) - l2); };
 
-  // The entries of this range: an open-addressing table of their tokens finds out
-  // whether one is listed twice (its probabilities add up); without repetitions,
-  // the usual case, each entry is put right by itself.
+  // The entries of this range: the first of each thread (mostly the only one) is loaded
+  // ahead of the long walk and looked at behind it.
+  int id[kPerThread];
+  float p[kPerThread];
+  const auto load_entry = [&](int i) {
+    const int k = tid + i * G;
+    id[i] = -1;
+    p[i] = 0.f;
+    if (k < t.K) {
+      id[i] = teacher_id(t, row * t.K + k, V);
+      p[i] = __ldg(probs + row * t.K + k);
+    }
+  };
+  load_entry(0);
   int size = 64;
   while (size < 2 * t.K) size *= 2;
-  for (int i = threadIdx.x; i < size; i += kThreads) seen[i] = -1;
-  __syncthreads();
+  for (int i = tid; i < size; i += G) seen[i] = -1;
+
+  const T* xp = x + c0;
+  if ((reinterpret_cast<uintptr_t>(xp) & 15) == (reinterpret_cast<uintptr_t>(dp) & 15) && !far) {
+    const uint64_t kk = f2_pack(k2, k2), nb = f2_pack(-base, -base), nl = f2_pack(-l2, -l2), cc = f2_pack(coef, coef);
+    const auto vec = [&](int i, const uint4& v) {
+      uint32_t o[4];
+#pragma unroll
+      for (int j = 0; j < Pairs<T>::N; ++j) {
+        const float2 e = f2_unpack(f2_add(f2_fma(Pairs<T>::get(v, j), kk, nb), nl));
+        const float2 r = f2_unpack(f2_mul(f2_pack(fast_exp2(e.x), fast_exp2(e.y)), cc));
+        if constexpr (sizeof(T) == 4) {
+          o[2 * j] = __float_as_uint(r.x);
+          o[2 * j + 1] = __float_as_uint(r.y);
+        } else {
+          o[j] = Pairs<T>::put(r);
+        }
+      }
+      *reinterpret_cast<uint4*>(dp + i) = make_uint4(o[0], o[1], o[2], o[3]);
+    };
+    constexpr int U = kBwdU<T, W>;
+    walk<U>(
+        xp, len, tid, G, [&](int i) { dp[i] = from_f<T>(coef * q(to_f(xp[i]))); },
+        [&](int i, int step, const uint4 (&v)[U]) {
+#pragma unroll
+          for (int u = 0; u < U; ++u) vec(i + u * step, v[u]);
+        },
+        vec);
+  } else {
+    for (int i = tid; i < len; i += G) dp[i] = from_f<T>(coef * q(to_f(xp[i])));
+  }
+#pragma unroll
+  for (int i = 1; i < kPerThread; ++i) load_entry(i);
+  if (W == 1) __syncwarp();
+  else __syncthreads();
+  // An open-addressing table of the tokens finds out whether one is listed twice (its
+  // probabilities add up).
   int twice = 0;
 #pragma unroll
   for (int i = 0; i < kPerThread; ++i) {
-    const int k = threadIdx.x + i * kThreads;
+    const int k = tid + i * G;
     if (k >= t.K) continue;
     if (id[i] < c0 || id[i] >= c1) id[i] = -1;
     ids[k] = id[i];
-    probs[k] = p[i];
-    if (id[i] >= 0) {
-      unsigned h = (unsigned)id[i] * 2654435761u;
-      for (h ^= h >> 15;; ++h) {
-        const int was = atomicCAS(&seen[h & (size - 1)], -1, id[i]);
-        if (was == -1) break;
-        if (was == id[i]) {
-          twice = 1;
-          break;
-        }
+    sp[k] = p[i];
+    if (id[i] < 0) continue;
+    unsigned h = (unsigned)id[i] * 2654435761u;
+    for (h ^= h >> 15;; ++h) {  // at most K of at least 2 K places are taken
+      const int was = atomicCAS(&seen[h & (size - 1)], -1, id[i]);
+      if (was == -1) break;
+      if (was == id[i]) {
+        twice = 1;
+        break;
       }
     }
   }
-  twice = __syncthreads_or(twice);  // also: the range is written
+  // also: the range is written
+  if (W == 1) {
+    twice = __any_sync(0xffffffffu, twice);
+    __syncwarp();
+  } else {
+    twice = __syncthreads_or(twice);
+  }
 #pragma unroll
   for (int i = 0; i < kPerThread; ++i) {
-    const int k = threadIdx.x + i * kThreads;
-    if (k >= t.K || id[i] < 0) continue;
+    const int k = tid + i * G;
+    if (id[i] < 0) continue;
     float all = p[i];
     if (twice) {
       bool first = true;
       for (int o = 0; o < k && first; ++o) first = ids[o] != id[i];
       if (!first) continue;
       for (int o = k + 1; o < t.K; ++o)
-        if (ids[o] == id[i]) all += probs[o];
+        if (ids[o] == id[i]) all += sp[o];
     }
     d[id[i]] = from_f<T>(coef * (q(to_f(x[id[i]])) - all));
   }
@@ -407,15 +587,25 @@ int row_split(int64_t n, int64_t V) {
   return s;
 }
 
+// A warp a row: enough rows for 12 warps an SM, lists that a warp holds, and rows short
+// enough that what a block spends on a row besides reading it (barriers, joins) shows.
+// 16384 fp16 rows: 8 KB each forward 32 us (103 us with a block a row), backward 42 us
+// (92 us); 32 KB 100 us (138 us) and 175 us (166 us); 64 KB 199 us (201 us) and 394 us
+// (320 us).
+bool warp_a_row(int64_t n, int64_t row_bytes, int K, int64_t most) {
+  return n >= 12 * (int64_t)num_sms() && K <= kWarpK && row_bytes <= most;
+}
+
 }  // namespace
 
-// logits (outer, inner, V); teacher (outer * inner, K).  Returns (row losses, counted
-// rows, row statistics, [loss, factor]); the last is filled for a sum or a mean
-// (reduction 1, 2) and left empty for 0.
+// logits (outer, inner, V); teacher (outer * inner, K).  Returns (row losses, row
+// statistics (N, 4) and the teacher's probabilities (N, K) for the backward -- the
+// latter left empty without `keep` --, [loss, factor]); the last is filled for a sum or
+// a mean (reduction 1, 2) and left empty for 0.
 std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> distill_fwd(const at::Tensor& logits,
                                                                        const at::Tensor& t_logits,
                                                                        const at::Tensor& t_ids, double temperature,
-                                                                       int64_t reduction) {
+                                                                       int64_t reduction, bool keep) {
   const Rows rows = make_rows(logits, "topk_distillation");
   const int64_t n = logits.size(0) * logits.size(1), V = logits.size(2);
   const Teacher t = make_teacher(t_logits, t_ids, logits, n, "topk_distillation");
@@ -423,56 +613,63 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> distill_fwd(const at:
   c10::cuda::CUDAGuard g(logits.device());
   bind_device(logits.get_device());
   auto f32 = logits.options().dtype(at::kFloat);
-  auto loss = at::empty({n}, f32), counted = at::empty({n}, f32), stats = at::empty({n, 2}, f32);
-  auto out = at::empty({reduction == 0 ? 0 : 2}, f32);
+  auto loss = at::empty({n}, f32), rest = at::empty({5 * n + (reduction == 0 ? 0 : 2)}, f32);
+  auto stats = rest.narrow(0, 0, 4 * n), out = rest.narrow(0, 5 * n, reduction == 0 ? 0 : 2);
+  float* counted = rest.data_ptr<float>() + 4 * n;
+  auto probs = at::empty({keep ? n : 0, t.K}, f32);
   if (n > 0) {
-    const int split = row_split(n, V);
     LRB_DISPATCH_FLOAT(logits.scalar_type(), T, [&] {
+      const bool warps = warp_a_row(n, V * sizeof(T), t.K, 32768);
+      const int split = warps ? 1 : row_split(n, V);
       cudaLaunchConfig_t cfg = {};
       cudaLaunchAttribute attr[1];
       attr[0].id = cudaLaunchAttributeClusterDimension;
       attr[0].val.clusterDim.x = (unsigned)split;
       attr[0].val.clusterDim.y = 1;
       attr[0].val.clusterDim.z = 1;
-      cfg.gridDim = dim3((unsigned)(n * split), 1, 1);
+      cfg.gridDim = dim3((unsigned)(warps ? (n + kWarps - 1) / kWarps : n * split), 1, 1);
       cfg.blockDim = dim3(kThreads, 1, 1);
       cfg.stream = stream();
       cfg.attrs = attr;
       cfg.numAttrs = 1;
-      LRB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, distill_fwd_kernel<T>, reinterpret_cast<const T*>(logits.data_ptr()), rows,
-                                        (int)V, t, (float)temperature, loss.data_ptr<float>(), counted.data_ptr<float>(),
-                                        reinterpret_cast<float2*>(stats.data_ptr<float>())));
+      LRB_CUDA_CHECK(cudaLaunchKernelEx(&cfg, warps ? distill_fwd_kernel<T, 1> : distill_fwd_kernel<T, kWarps>,
+                                        reinterpret_cast<const T*>(logits.data_ptr()), rows, n, (int)V, t,
+                                        (float)temperature, loss.data_ptr<float>(), counted,
+                                        reinterpret_cast<RowStats*>(stats.data_ptr<float>()),
+                                        keep ? probs.data_ptr<float>() : (float*)nullptr));
     });
   }
   if (reduction != 0) {
-    reduce_rows_kernel<<<1, 1024, 0, stream()>>>(loss.data_ptr<float>(), counted.data_ptr<float>(), n,
-                                                 reduction == 2 ? 1 : 0, out.data_ptr<float>());
+    reduce_rows_kernel<<<1, 1024, 0, stream()>>>(loss.data_ptr<float>(), counted, n, reduction == 2 ? 1 : 0,
+                                                 out.data_ptr<float>());
     LRB_LAUNCH_CHECK();
   }
-  return {loss, counted, stats, out};
+  return {loss, stats, probs, out};
 }
 
 // Gradient of the logits (contiguous, their shape): `g` fp32, one value for each row
 // (g_per_row) or a single one that is multiplied by `factor`.
-at::Tensor distill_bwd(const at::Tensor& logits, const at::Tensor& t_logits, const at::Tensor& t_ids,
-                       double temperature, const at::Tensor& stats, const at::Tensor& g, bool g_per_row,
-                       const at::Tensor& factor) {
+at::Tensor distill_bwd(const at::Tensor& logits, const at::Tensor& t_ids, double temperature, const at::Tensor& stats,
+                       const at::Tensor& probs, const at::Tensor& g, bool g_per_row, const at::Tensor& factor) {
   const Rows rows = make_rows(logits, "topk_distillation backward");
   const int64_t n = logits.size(0) * logits.size(1), V = logits.size(2);
-  const Teacher t = make_teacher(t_logits, t_ids, logits, n, "topk_distillation backward");
+  const Teacher t = make_teacher(probs, t_ids, logits, n, "topk_distillation backward");
   LRB_CHECK(g.is_cuda() && g.scalar_type() == at::kFloat && g.is_contiguous() && g.numel() == (g_per_row ? n : 1) &&
-                stats.scalar_type() == at::kFloat && stats.is_contiguous() && stats.numel() == 2 * n &&
+                stats.scalar_type() == at::kFloat && stats.is_contiguous() && stats.numel() == 4 * n &&
+                probs.scalar_type() == at::kFloat &&
                 (g_per_row || (factor.is_cuda() && factor.scalar_type() == at::kFloat && factor.numel() >= 1)),
             "topk_distillation backward: bad gradient or statistics");
   c10::cuda::CUDAGuard guard(logits.device());
   bind_device(logits.get_device());
   auto dx = at::empty(logits.sizes(), logits.options());
   if (n == 0) return dx;
-  const int split = row_split(n, V);
   LRB_DISPATCH_FLOAT(logits.scalar_type(), T, [&] {
-    distill_bwd_kernel<T><<<(unsigned)(n * split), kThreads, 0, stream()>>>(
-        reinterpret_cast<const T*>(logits.data_ptr()), rows, (int)V, t, (float)temperature,
-        reinterpret_cast<const float2*>(stats.data_ptr<float>()), g.data_ptr<float>(), g_per_row ? 1 : 0,
+    const bool warps = warp_a_row(n, V * sizeof(T), t.K, 16384);
+    const int split = warps ? 1 : row_split(n, V);
+    const auto k = warps ? distill_bwd_kernel<T, 1> : distill_bwd_kernel<T, kWarps>;
+    k<<<(unsigned)(warps ? (n + kWarps - 1) / kWarps : n * split), kThreads, 0, stream()>>>(
+        reinterpret_cast<const T*>(logits.data_ptr()), rows, n, (int)V, t, (float)temperature, probs.data_ptr<float>(),
+        reinterpret_cast<const RowStats*>(stats.data_ptr<float>()), g.data_ptr<float>(), g_per_row ? 1 : 0,
         g_per_row ? nullptr : factor.data_ptr<float>(), reinterpret_cast<T*>(dx.data_ptr()), split);
   });
   LRB_LAUNCH_CHECK();

@@ -12,7 +12,7 @@ row without entries has loss 0, gradient 0 and is left out of the mean.  A token
 listed twice has the sum of its probabilities.  The teacher gets no gradient.
 
 CUDA (``csrc/kernels/distill.cu``): the forward reads the logits once and keeps
-two numbers a row; the backward reads them once and writes the gradient; fp32
+four numbers a row and the teacher's probabilities; the backward reads them once and writes the gradient; fp32
 arithmetic for bf16, fp16 and fp32 logits.  The full-vocabulary form of the
 same loss is ``VerificationDistillation.temperature_scaled_loss``.
 """
@@ -54,17 +54,17 @@ def _plain(x, teacher, ids, T, reduction):
 class _TopkDistillFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, teacher, ids, T, reduction):
-        rows, _, stats, out = native().distill_fwd(x, teacher, ids, T, reduction)
-        ctx.save_for_backward(x, teacher, ids, stats, out)
+        rows, stats, probs, out = native().distill_fwd(x, teacher, ids, T, reduction, True)
+        ctx.save_for_backward(x, ids, stats, probs, out)
         ctx.T, ctx.reduction = T, reduction
         return rows if reduction == 0 else out[0]
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
-        x, teacher, ids, stats, out = ctx.saved_tensors
+        x, ids, stats, probs, out = ctx.saved_tensors
         per_row = ctx.reduction == 0
-        dx = native().distill_bwd(x, teacher, ids, ctx.T, stats, g.float().contiguous(), per_row,
+        dx = native().distill_bwd(x, ids, ctx.T, stats, probs, g.float().contiguous(), per_row,
                                   stats if per_row else out[1:])
         return dx, None, None, None, None
 
@@ -104,6 +104,6 @@ def topk_distillation(logits: torch.Tensor, teacher_logits: torch.Tensor, teache
     if x.requires_grad and torch.is_grad_enabled():
         out = _TopkDistillFn.apply(x, teacher, ids, T, code)
     else:
-        rows, _, _, out = native().distill_fwd(x, teacher, ids, T, code)
+        rows, _, _, out = native().distill_fwd(x, teacher, ids, T, code, False)
         out = rows if code == 0 else out[0]
     return out.view(lead) if reduction == "none" else out

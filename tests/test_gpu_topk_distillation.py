@@ -253,3 +253,14 @@ def test_cuda_refusals():
         ops.topk_distillation(x, teacher.repeat(1, 600), ids.repeat(1, 600))
     with pytest.raises(RuntimeError, match="one CUDA device"):
         ops.topk_distillation(x, teacher.cpu(), ids)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("N,V,K", [(2500, 301, 5), (1776, 1024, 128), (1777, 16384, 33), (1800, 515, 129)])
+def test_many_rows(dtype, N, V, K):
+    """Rows by warps (lists up to 128 entries, short rows) and by blocks; a list with repetitions."""
+    x, teacher, ids = _inputs(N, V, K, dtype, N)
+    ids[7] = ids[7, 0]
+    ids[8, -1] = ids[8, 0]
+    _compare(x, teacher, ids, 1.3, "none", torch.randn(N, device="cuda"))
