@@ -1,0 +1,158 @@
+// Autograd nodes of the vocabulary operators (embedding.cu, linear_ce.cu, distill.cu).
+// They are recorded and run without the interpreter: for the small calls of these
+// operators a Python-level node costs more than the kernels (256 tokens of 64 fp16
+// columns, forward and gradient: 87 us with Python nodes).
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/extension.h>
+
+#include <memory>
+#include <tuple>
+
+namespace lrb {
+
+at::Tensor embedding_fwd(const at::Tensor&, const at::Tensor&, double);
+at::Tensor embedding_bwd(const at::Tensor&, const at::Tensor&, int64_t, int64_t, double);
+std::tuple<at::Tensor, at::Tensor, at::Tensor> linear_ce_fwd(const at::Tensor&, const at::Tensor&, const at::Tensor&,
+                                                             int64_t, int64_t);
+std::tuple<at::Tensor, at::Tensor> linear_ce_bwd(const at::Tensor&, const at::Tensor&, const at::Tensor&, int64_t,
+                                                 const at::Tensor&, const at::Tensor&, bool, const at::Tensor&, int64_t,
+                                                 bool, bool);
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> distill_fwd(const at::Tensor&, const at::Tensor&,
+                                                                       const at::Tensor&, double, int64_t, bool);
+at::Tensor distill_bwd(const at::Tensor&, const at::Tensor&, double, const at::Tensor&, const at::Tensor&,
+                       const at::Tensor&, bool, const at::Tensor&);
+
+namespace {
+
+using torch::autograd::AutogradContext;
+using torch::autograd::Function;
+using torch::autograd::Variable;
+using torch::autograd::variable_list;
+
+// Gradients that have no gradient of their own: differentiating them raises.
+variable_list once(const char* name, variable_list grads) {
+  if (!at::GradMode::is_enabled()) return grads;
+  for (auto& g : grads)
+    if (g.defined()) g = g.detach().requires_grad_(true);
+  auto err = std::make_shared<torch::autograd::DelayedError>(std::string(name) + " is differentiable once",
+                                                             (int64_t)grads.size());
+  return (*err)(std::move(grads));
+}
+
+at::Tensor unit_columns(const at::Tensor& t) { return t.stride(-1) == 1 || t.size(-1) <= 1 ? t : t.contiguous(); }
+
+struct EmbeddingGradFn;
+
+struct EmbeddingFn : public Function<EmbeddingFn> {
+  static Variable forward(AutogradContext* ctx, const Variable& w, const Variable& ids, double scale, int64_t padding) {
+    ctx->save_for_backward({ids});
+    ctx->saved_data["rows"] = w.size(0);
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["padding"] = padding;
+    return embedding_fwd(ids, w, scale);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g);
+};
+
+// The gradient is linear in dy; its own gradient is the lookup (zero at the padding
+// token and at ids outside the table).
+struct EmbeddingGradFn : public Function<EmbeddingGradFn> {
+  static Variable forward(AutogradContext* ctx, const Variable& dy, const Variable& ids, int64_t rows, double scale,
+                          int64_t padding) {
+    ctx->save_for_backward({ids});
+    ctx->saved_data["rows"] = rows;
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["padding"] = padding;
+    return embedding_bwd(unit_columns(dy), ids, rows, padding, scale);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    const auto ids = ctx->get_saved_variables()[0];
+    const int64_t padding = ctx->saved_data["padding"].toInt();
+    const auto out = EmbeddingFn::apply(g[0].contiguous(), ids, ctx->saved_data["scale"].toDouble(), padding);
+    const auto kept = ids.ge(0).logical_and(ids.lt(ctx->saved_data["rows"].toInt())).logical_and(ids.ne(padding));
+    return {at::where(kept.unsqueeze(1), out, at::zeros({}, out.options())), Variable(), Variable(), Variable(),
+            Variable()};
+  }
+};
+
+variable_list EmbeddingFn::backward(AutogradContext* ctx, variable_list g) {
+  const auto ids = ctx->get_saved_variables()[0];
+  const int64_t rows = ctx->saved_data["rows"].toInt(), padding = ctx->saved_data["padding"].toInt();
+  const double scale = ctx->saved_data["scale"].toDouble();
+  const auto dw = at::GradMode::is_enabled() ? EmbeddingGradFn::apply(g[0], ids, rows, scale, padding)
+                                             : embedding_bwd(unit_columns(g[0]), ids, rows, padding, scale);
+  return {dw, Variable(), Variable(), Variable()};
+}
+
+struct LinearCEFn : public Function<LinearCEFn> {
+  static Variable forward(AutogradContext* ctx, const Variable& h, const Variable& w, const Variable& targets,
+                          int64_t ignore, int64_t reduction, int64_t piece) {
+    auto [rows, stats, out] = linear_ce_fwd(h, w, targets, ignore, reduction);
+    ctx->save_for_backward({h, w, targets, stats, out});
+    ctx->saved_data["ignore"] = ignore;
+    ctx->saved_data["per_row"] = reduction == 0;
+    ctx->saved_data["piece"] = piece;
+    return reduction == 0 ? rows : out.select(0, 0);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    const auto s = ctx->get_saved_variables();
+    const bool per_row = ctx->saved_data["per_row"].toBool(), need_h = ctx->needs_input_grad(0),
+               need_w = ctx->needs_input_grad(1);
+    at::Tensor dh, dw;
+    {
+      at::AutoGradMode off(false);
+      std::tie(dh, dw) = linear_ce_bwd(s[0], s[1], s[2], ctx->saved_data["ignore"].toInt(), s[3],
+                                       g[0].to(at::kFloat).contiguous(), per_row,
+                                       per_row ? s[3] : s[4].narrow(0, 1, 1), ctx->saved_data["piece"].toInt(), need_h,
+                                       need_w);
+    }
+    return once("piecewise_linear_cross_entropy", {need_h ? dh : Variable(), need_w ? dw : Variable(), Variable(),
+                                                   Variable(), Variable(), Variable()});
+  }
+};
+
+struct DistillFn : public Function<DistillFn> {
+  static Variable forward(AutogradContext* ctx, const Variable& x, const Variable& teacher, const Variable& ids,
+                          double temperature, int64_t reduction) {
+    auto [rows, stats, probs, out] = distill_fwd(x, teacher, ids, temperature, reduction, true);
+    ctx->save_for_backward({x, ids, stats, probs, out});
+    ctx->saved_data["temperature"] = temperature;
+    ctx->saved_data["per_row"] = reduction == 0;
+    return reduction == 0 ? rows : out.select(0, 0);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    const auto s = ctx->get_saved_variables();
+    const bool per_row = ctx->saved_data["per_row"].toBool();
+    at::Tensor dx;
+    {
+      at::AutoGradMode off(false);
+      dx = distill_bwd(s[0], s[1], ctx->saved_data["temperature"].toDouble(), s[2], s[3],
+                       g[0].to(at::kFloat).contiguous(), per_row, per_row ? s[2] : s[4].narrow(0, 1, 1));
+    }
+    return once("topk_distillation", {dx, Variable(), Variable(), Variable(), Variable()});
+  }
+};
+
+bool tracked(const at::Tensor& t) { return at::GradMode::is_enabled() && t.requires_grad(); }
+
+}  // namespace
+
+at::Tensor embedding(const at::Tensor& ids, const at::Tensor& w, double scale, int64_t padding) {
+  return tracked(w) ? EmbeddingFn::apply(w, ids, scale, padding) : embedding_fwd(ids, w, scale);
+}
+
+at::Tensor piecewise_linear_ce(const at::Tensor& h, const at::Tensor& w, const at::Tensor& targets, int64_t ignore,
+                               int64_t reduction, int64_t piece) {
+  if (tracked(h) || tracked(w)) return LinearCEFn::apply(h, w, targets, ignore, reduction, piece);
+  auto [rows, stats, out] = linear_ce_fwd(h, w, targets, ignore, reduction);
+  return reduction == 0 ? rows : out.select(0, 0);
+}
+
+at::Tensor topk_distillation(const at::Tensor& x, const at::Tensor& teacher, const at::Tensor& ids, double temperature,
+                             int64_t reduction) {
+  if (tracked(x)) return DistillFn::apply(x, teacher, ids, temperature, reduction);
+  auto [rows, stats, probs, out] = distill_fwd(x, teacher, ids, temperature, reduction, false);
+  return reduction == 0 ? rows : out.select(0, 0);
+}
+
+}  // namespace lrb

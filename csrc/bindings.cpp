@@ -24,19 +24,11 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> ce_fwd(const at::Tensor&, const a
 at::Tensor ce_bwd(const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&, int64_t);
 at::Tensor ce_bwd_vocab_shard(const at::Tensor&, const at::Tensor&, const at::Tensor&, const at::Tensor&, int64_t);
 // embedding.cu
-at::Tensor embedding_fwd(const at::Tensor&, const at::Tensor&, double);
 at::Tensor embedding_bwd(const at::Tensor&, const at::Tensor&, int64_t, int64_t, double);
-// linear_ce.cu
-std::tuple<at::Tensor, at::Tensor, at::Tensor> linear_ce_fwd(const at::Tensor&, const at::Tensor&, const at::Tensor&,
-                                                             int64_t, int64_t);
-std::tuple<at::Tensor, at::Tensor> linear_ce_bwd(const at::Tensor&, const at::Tensor&, const at::Tensor&, int64_t,
-                                                 const at::Tensor&, const at::Tensor&, bool, const at::Tensor&, int64_t,
-                                                 bool, bool);
-// distill.cu
-std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> distill_fwd(const at::Tensor&, const at::Tensor&,
-                                                                       const at::Tensor&, double, int64_t, bool);
-at::Tensor distill_bwd(const at::Tensor&, const at::Tensor&, double, const at::Tensor&, const at::Tensor&,
-                       const at::Tensor&, bool, const at::Tensor&);
+// autograd.cpp
+at::Tensor embedding(const at::Tensor&, const at::Tensor&, double, int64_t);
+at::Tensor piecewise_linear_ce(const at::Tensor&, const at::Tensor&, const at::Tensor&, int64_t, int64_t, int64_t);
+at::Tensor topk_distillation(const at::Tensor&, const at::Tensor&, const at::Tensor&, double, int64_t);
 // routing.cu
 std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> route_slots(const at::Tensor&, int64_t, int64_t, int64_t);
 std::tuple<at::Tensor, at::Tensor, at::Tensor> softmax_topk_fwd(const at::Tensor&, int64_t);
@@ -161,12 +153,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("ce_fwd", &lrb::ce_fwd);
   m.def("ce_bwd", &lrb::ce_bwd);
   m.def("ce_bwd_vocab_shard", &lrb::ce_bwd_vocab_shard);
-  m.def("embedding_fwd", &lrb::embedding_fwd, "scale * w[ids]");
-  m.def("embedding_bwd", &lrb::embedding_bwd, "dense gradient of the table, by sorted tokens");
-  m.def("linear_ce_fwd", &lrb::linear_ce_fwd, "softmax cross entropy of h w^T without the logits");
-  m.def("linear_ce_bwd", &lrb::linear_ce_bwd, "its gradients, one piece of the vocabulary at a time");
-  m.def("distill_fwd", &lrb::distill_fwd, "distillation from a teacher's top logits");
-  m.def("distill_bwd", &lrb::distill_bwd);
+  m.def("embedding", &lrb::embedding, "scale * w[ids]; its gradient by sorted tokens");
+  m.def("embedding_bwd", &lrb::embedding_bwd, "dense gradient of the table");
+  m.def("piecewise_linear_ce", &lrb::piecewise_linear_ce,
+        "softmax cross entropy of h w^T without the logits; its gradients in pieces of the vocabulary");
+  m.def("topk_distillation", &lrb::topk_distillation, "distillation from a teacher's top logits");
   m.def("route_slots", &lrb::route_slots, "capacity slots, owner ranks and per-expert counts of routed assignments");
   m.def("softmax_topk_fwd", &lrb::softmax_topk_fwd);
   m.def("chunk_mean_pool_fwd", &lrb::chunk_mean_pool_fwd);

@@ -434,7 +434,7 @@ template <typename IdT>
 void launch_sort(const at::Tensor& ids, const SortArgs& a, int blocks) {
   auto k = sort_tokens_kernel<IdT>;
   const int smem = ((kSortWarps + 2) << a.bits) * (int)sizeof(int);
-  LRB_CUDA_CHECK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  if (smem > 48 * 1024) LRB_CUDA_CHECK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
   if (blocks > 8) LRB_CUDA_CHECK(cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];

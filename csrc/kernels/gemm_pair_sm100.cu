@@ -1259,6 +1259,30 @@ int gemm_pair_slices(int64_t M, int64_t N, int64_t K, int dev) {
   return (int)std::max<int64_t>(1, std::min<int64_t>({max_pairs(dev) / std::max<int64_t>(tiles, 1), nk / 8, 64}));
 }
 
+// Vocabulary rows at a time for the backward of the linear cross entropy, whose three
+// products a piece run in waves of one tile a CTA pair: the width whose waves cost
+// least over all pieces, among those whose 16-bit (n, width) buffer stays below `bytes`
+// (at least 1024 rows).  N = 16384, V = 32000, d = 2048: 4 pieces of 8192 rows leave the
+// 256 tiles of each piece's dw 13 % short of whole waves of 74; 5 of 6912 (216 tiles) 3 %.
+int64_t gemm_pair_ce_piece(int64_t n, int64_t V, int64_t d, int64_t bytes, int dev) {
+  const int64_t pairs = max_pairs(dev);
+  const auto up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
+  const int64_t tm = up(n, 256), td = up(d, 256), most = std::max<int64_t>(4, std::min(up(V, 256), bytes / (512 * std::max<int64_t>(n, 1))));
+  // the time of a launch in steps of one K element of a tile (6 ns)
+  constexpr int64_t kLaunch = 1000;
+  const auto cost = [&](int64_t w) {
+    const int64_t tv = up(w, 256), sh = gemm_pair_slices(n, d, w, dev), sw = gemm_pair_slices(w, d, n, dev);
+    return up(tm * tv, pairs) * d + up(tm * td * sh, pairs) * up(w, sh) + up(tv * td * sw, pairs) * up(n, sw) + 3 * kLaunch;
+  };
+  int64_t best = most, least = -1;
+  for (int64_t r = most; r >= std::max<int64_t>(4, most / 4); --r) {
+    const int64_t w = 256 * r, full = V / w, last = V - full * w;
+    const int64_t c = full * cost(w) + (last > 0 ? cost(last) : 0);
+    if (least < 0 || c < least) least = c, best = r;
+  }
+  return 256 * best;
+}
+
 // C (S, M, N) fp32 (+)= the product over each of `splits` <= S ranges of K, slice by
 // slice (no two of them meet in one element, so nothing depends on their order); or,
 // with a 16-bit 2-D C, C = alpha_dev * A B in one piece.

@@ -27,6 +27,7 @@ void gemm_pair_lse(const at::Tensor&, const at::Tensor&, const at::Tensor&, at::
 void gemm_pair_ce_grad(const at::Tensor&, const at::Tensor&, const at::Tensor&, int64_t, const at::Tensor&,
                        const at::Tensor&, at::Tensor&);
 int gemm_pair_slices(int64_t, int64_t, int64_t, int);
+int64_t gemm_pair_ce_piece(int64_t, int64_t, int64_t, int64_t, int);
 void gemm_pair_sliced(const at::Tensor&, const at::Tensor&, bool, bool, at::Tensor&, int, bool, const float*);
 // distill.cu
 void reduce_rows(const float*, const float*, int64_t, bool, float*, cudaStream_t);
@@ -175,7 +176,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> linear_ce_fwd(const at::Tensor& h
 }
 
 // (dh, dw), each empty where it is not asked for.  `g` fp32: one value for each row,
-// or a single one that is multiplied by `factor`.  `piece`: vocabulary rows at a time.
+// or a single one that is multiplied by `factor`.  `piece`: vocabulary rows at a time, a
+// multiple of 8; 0: a buffer of at most 256 MB or 1024 rows.
 std::tuple<at::Tensor, at::Tensor> linear_ce_bwd(const at::Tensor& h, const at::Tensor& w, const at::Tensor& targets,
                                                  int64_t ignore, const at::Tensor& stats, const at::Tensor& g,
                                                  bool g_per_row, const at::Tensor& factor, int64_t piece, bool need_h,
@@ -186,7 +188,7 @@ std::tuple<at::Tensor, at::Tensor> linear_ce_bwd(const at::Tensor& h, const at::
                 stats.scalar_type() == at::kFloat && stats.is_contiguous() && stats.numel() == 2 * n &&
                 (g_per_row || (factor.is_cuda() && factor.scalar_type() == at::kFloat && factor.numel() >= 1)),
             "linear cross entropy backward: bad gradient or statistics");
-  LRB_CHECK(piece >= 8 && piece % 8 == 0, "linear cross entropy backward: piece must be a positive multiple of 8");
+  LRB_CHECK(piece >= 0 && piece % 8 == 0, "linear cross entropy backward: piece must be a multiple of 8");
   c10::cuda::CUDAGuard guard(h.device());
   const int dev = h.get_device();
   bind_device(dev);
@@ -202,6 +204,7 @@ std::tuple<at::Tensor, at::Tensor> linear_ce_bwd(const at::Tensor& h, const at::
       g_per_row ? nullptr : factor.data_ptr<float>(), normalise ? 1 : 0, scale.data_ptr<float>(),
       scale.data_ptr<float>() + n);
   LRB_LAUNCH_CHECK();
+  if (piece == 0) piece = gemm_pair_ce_piece(n, V, d, 256 << 20, dev);
   piece = std::min(piece, (V + 7) / 8 * 8);
   auto buf = at::empty({n, piece}, h.options());
   // dh: K ranges of the first piece as slices, later pieces added to them

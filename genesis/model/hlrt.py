@@ -244,16 +244,21 @@ class HLRT(StatefulModule):
         kv_cache: Optional[Any] = None,
         position_offset: int = 0,
         labels: Optional[torch.Tensor] = None,
+        lm_loss: str = "rows",
+        lm_reduction: str = "mean",
     ) -> Dict[str, Any]:
         """``labels`` (an extension; per-position targets, ``-100`` ignored): the
         head and the token cross-entropy run chunk by chunk
         (``llm_research_b200.ops.loss.linear_cross_entropy``) and the output
-        carries ``lm_loss`` instead of the ``(B, S, vocab)`` logits."""
+        carries ``lm_loss`` instead of the ``(B, S, vocab)`` logits.  ``lm_loss =
+        "pieces"`` runs them in pieces of the vocabulary instead
+        (``piecewise_linear_cross_entropy``: no logits kept), with ``lm_reduction``
+        ``"mean"``, ``"sum"`` or ``"none"`` (one loss for each position)."""
         x = self.embeddings(input_ids)
         t1 = self.tier1(x, attention_mask=attention_mask, kv_cache=kv_cache, position_offset=position_offset)
         return self.forward_after_tier1(t1, attention_mask=attention_mask,
                                         return_tier_activations=return_tier_activations, kv_cache=kv_cache,
-                                        labels=labels)
+                                        labels=labels, lm_loss=lm_loss, lm_reduction=lm_reduction)
 
     def forward_after_tier1(
         self,
@@ -262,9 +267,17 @@ class HLRT(StatefulModule):
         return_tier_activations: bool = False,
         kv_cache: Optional[Any] = None,
         labels: Optional[torch.Tensor] = None,
+        lm_loss: str = "rows",
+        lm_reduction: str = "mean",
     ) -> Dict[str, Any]:
         """Everything after the Tier-1 trunk: gates, Tiers 2/3, plan conditioning and
         the head (the last pipeline stage runs this on the trunk's output)."""
+        if lm_loss not in ("rows", "pieces"):
+            raise ValueError(f"lm_loss must be 'rows' or 'pieces', got {lm_loss!r}")
+        if lm_loss == "rows" and lm_reduction != "mean":
+            raise ValueError("lm_reduction other than 'mean' needs lm_loss='pieces'")
+        if lm_loss == "pieces" and self._vocab_parallel_group is not None:
+            raise ValueError("lm_loss='pieces' does not split the vocabulary over a tensor-parallel group")
         B, S = t1.shape[0], t1.shape[1]
         acts: Dict[str, Any] = {}
         if return_tier_activations:
@@ -321,14 +334,17 @@ class HLRT(StatefulModule):
 
         h = self.output_norm(t1)
         if labels is not None:
-            from llm_research_b200.ops.loss import linear_cross_entropy, vocab_parallel_linear_cross_entropy
+            from llm_research_b200.ops.loss import (linear_cross_entropy, piecewise_linear_cross_entropy,
+                                                    vocab_parallel_linear_cross_entropy)
 
             w = self.output_proj.weight if self.output_proj is not None else self.embeddings.weight
-            if self._vocab_parallel_group is not None:
-                lm_loss = vocab_parallel_linear_cross_entropy(h, w, labels, self._vocab_parallel_group)
+            if lm_loss == "pieces":
+                token_loss = piecewise_linear_cross_entropy(h, w, labels, reduction=lm_reduction)
+            elif self._vocab_parallel_group is not None:
+                token_loss = vocab_parallel_linear_cross_entropy(h, w, labels, self._vocab_parallel_group)
             else:
-                lm_loss = linear_cross_entropy(h, w, labels)
-            out = {"logits": None, "lm_loss": lm_loss, "hidden_states": h, "aux_loss": aux}
+                token_loss = linear_cross_entropy(h, w, labels)
+            out = {"logits": None, "lm_loss": token_loss, "hidden_states": h, "aux_loss": aux}
         else:
             out = {"logits": self._head(h), "hidden_states": h, "aux_loss": aux}
         if return_tier_activations:

@@ -44,7 +44,9 @@ def ntp_objective(models: Dict[str, nn.Module], ctx: TrainingContext, batch: Any
         input_ids = input_ids.to(device, non_blocking=True)
     if batch.get("fused_lm_loss", False):  # extension: chunked head + CE, no full logits
         targets = torch.cat([input_ids[:, 1:], input_ids.new_full((input_ids.shape[0], 1), -100)], dim=1)
-        out = model(input_ids, labels=targets)
+        # "pieces": in pieces of the vocabulary instead of chunks of rows
+        how = {"lm_loss": "pieces"} if batch["fused_lm_loss"] == "pieces" else {}
+        out = model(input_ids, labels=targets, **how)
         loss = out["lm_loss"]
     else:
         out = model(input_ids)

@@ -4,7 +4,8 @@
 shared space, the verifier side detached.  ``temperature_scaled_loss``:
 ``T² · KL(softmax(v/T) ‖ softmax(g/T))`` with batch-mean reduction.
 ``forward`` returns the MSE term (the KL term is called explicitly when
-logits exist).
+logits exist).  ``topk_loss`` (an extension) is the KL term against a stored
+list of the verifier's top logits (``llm_research_b200.ops.topk_distillation``).
 """
 
 from __future__ import annotations
@@ -12,6 +13,8 @@ from __future__ import annotations
 import torch
 import torch.nn as nn
 import torch.nn.functional as F
+
+from llm_research_b200 import ops
 
 
 class VerificationDistillation(nn.Module):
@@ -35,6 +38,13 @@ class VerificationDistillation(nn.Module):
         g = F.log_softmax(g_logits.float() / temperature, dim=-1)
         v = F.softmax(v_logits.float() / temperature, dim=-1).detach()
         return F.kl_div(g, v, reduction="batchmean") * (temperature ** 2)
+
+    def topk_loss(self, g_logits: torch.Tensor, v_top_logits: torch.Tensor, v_top_ids: torch.Tensor,
+                  temperature: float = 2.0) -> torch.Tensor:
+        """``T² · KL`` of the generator's ``(..., V)`` logits against the verifier's
+        ``(..., K)`` largest logits and their token ids (id -1: no entry), averaged over
+        the rows that have entries."""
+        return ops.topk_distillation(g_logits, v_top_logits, v_top_ids, temperature)
 
     def forward(self, generator_hidden: torch.Tensor, verifier_hidden: torch.Tensor) -> torch.Tensor:
         return self.distillation_loss(generator_hidden, verifier_hidden)

@@ -51,24 +51,6 @@ def _plain(x, teacher, ids, T, reduction):
     return rows.sum() if reduction == "sum" else rows.sum() / some.sum().clamp(min=1)
 
 
-class _TopkDistillFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, teacher, ids, T, reduction):
-        rows, stats, probs, out = native().distill_fwd(x, teacher, ids, T, reduction, True)
-        ctx.save_for_backward(x, ids, stats, probs, out)
-        ctx.T, ctx.reduction = T, reduction
-        return rows if reduction == 0 else out[0]
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, g):
-        x, ids, stats, probs, out = ctx.saved_tensors
-        per_row = ctx.reduction == 0
-        dx = native().distill_bwd(x, ids, ctx.T, stats, probs, g.float().contiguous(), per_row,
-                                  stats if per_row else out[1:])
-        return dx, None, None, None, None
-
-
 def topk_distillation(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_ids: torch.Tensor,
                       temperature: float = 1.0, reduction: str = "mean") -> torch.Tensor:
     """``logits`` ``(..., V)``; ``teacher_logits``, ``teacher_ids`` ``(..., K)`` with
@@ -100,10 +82,5 @@ def topk_distillation(logits: torch.Tensor, teacher_logits: torch.Tensor, teache
     x = logits if logits.dim() == 3 else logits.unsqueeze(0) if logits.dim() == 2 else logits.reshape(1, -1, V)
     if x.stride(-1) != 1 and V > 1:
         x = x.contiguous()
-    teacher, ids, code = teacher.contiguous(), ids.contiguous(), _REDUCTIONS[reduction]
-    if x.requires_grad and torch.is_grad_enabled():
-        out = _TopkDistillFn.apply(x, teacher, ids, T, code)
-    else:
-        rows, _, _, out = native().distill_fwd(x, teacher, ids, T, code, False)
-        out = rows if code == 0 else out[0]
+    out = native().topk_distillation(x, teacher.contiguous(), ids.contiguous(), T, _REDUCTIONS[reduction])
     return out.view(lead) if reduction == "none" else out

@@ -24,43 +24,6 @@ from llm_research_b200._ext import native
 _DTYPES = (torch.bfloat16, torch.float16, torch.float32)
 
 
-class _EmbeddingFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, weight, ids, scale, padding):
-        ctx.save_for_backward(ids)
-        ctx.rows, ctx.scale, ctx.padding = weight.shape[0], scale, padding
-        return native().embedding_fwd(ids, weight, scale)
-
-    @staticmethod
-    def backward(ctx, dy):
-        ids, = ctx.saved_tensors
-        if torch.is_grad_enabled():  # create_graph
-            return _EmbeddingGradFn.apply(dy, ids, ctx.rows, ctx.scale, ctx.padding), None, None, None
-        return _grad(dy, ids, ctx.rows, ctx.scale, ctx.padding), None, None, None
-
-
-def _grad(dy, ids, rows, scale, padding):
-    return native().embedding_bwd(dy if dy.stride(-1) == 1 else dy.contiguous(), ids, rows, padding, scale)
-
-
-class _EmbeddingGradFn(torch.autograd.Function):
-    """The gradient is linear in ``dy``; its own gradient is the lookup (zero at the
-    padding token and at ids outside the table)."""
-
-    @staticmethod
-    def forward(ctx, dy, ids, rows, scale, padding):
-        ctx.save_for_backward(ids)
-        ctx.rows, ctx.scale, ctx.padding = rows, scale, padding
-        return _grad(dy, ids, rows, scale, padding)
-
-    @staticmethod
-    def backward(ctx, g):
-        ids, = ctx.saved_tensors
-        out = _EmbeddingFn.apply(g.contiguous(), ids, ctx.scale, ctx.padding)
-        kept = (ids >= 0) & (ids < ctx.rows) & (ids != ctx.padding)
-        return torch.where(kept[:, None], out, torch.zeros_like(out)), None, None, None, None
-
-
 def embedding(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0,
               padding_idx: Optional[int] = None) -> torch.Tensor:
     """``scale * weight[ids]``, shape ``(*ids.shape, d)``; ``ids`` int64 or int32 of any
@@ -86,8 +49,5 @@ def embedding(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0,
         flat = flat.contiguous()
     if weight.stride(1) != 1:
         weight = weight.contiguous()
-    if weight.requires_grad and torch.is_grad_enabled():
-        out = _EmbeddingFn.apply(weight, flat, scale, -1 if padding_idx is None else padding_idx)
-    else:
-        out = native().embedding_fwd(flat, weight, scale)
+    out = native().embedding(flat, weight, scale, -1 if padding_idx is None else padding_idx)
     return out.view(*ids.shape, weight.shape[1])

@@ -142,34 +142,6 @@ def linear_cross_entropy(h: torch.Tensor, w: torch.Tensor, targets: torch.Tensor
 
 # ------------------------------------------------ linear + CE in pieces of the vocabulary
 _REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
-_PIECE_BYTES = 256 << 20
-
-
-def _vocab_piece(n: int, V: int) -> int:
-    """Vocabulary rows at a time: a 16-bit ``(n, piece)`` buffer of at most about 256 MB
-    (at least 1024 wide), the vocabulary divided evenly into multiples of 256."""
-    most = max(1024, _PIECE_BYTES // (2 * max(n, 1)))
-    pieces = -(-V // most)
-    return (-(-V // pieces) + 255) // 256 * 256
-
-
-class _PiecewiseLinearCEFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, h, w, targets, ignore_index, reduction, piece):
-        rows, stats, out = native().linear_ce_fwd(h, w, targets, ignore_index, reduction)
-        ctx.save_for_backward(h, w, targets, stats, out)
-        ctx.ignore_index, ctx.reduction, ctx.piece = ignore_index, reduction, piece
-        return rows if reduction == 0 else out[0]
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, g):
-        h, w, targets, stats, out = ctx.saved_tensors
-        per_row = ctx.reduction == 0
-        need_h, need_w = ctx.needs_input_grad[:2]
-        dh, dw = native().linear_ce_bwd(h, w, targets, ctx.ignore_index, stats, g.float().contiguous(), per_row,
-                                        stats if per_row else out[1:], ctx.piece, need_h, need_w)
-        return dh if need_h else None, dw if need_w else None, None, None, None, None
 
 
 def piecewise_linear_cross_entropy(h: torch.Tensor, w: torch.Tensor, targets: torch.Tensor, ignore_index: int = -100,
@@ -183,7 +155,7 @@ def piecewise_linear_cross_entropy(h: torch.Tensor, w: torch.Tensor, targets: to
     multiple of 8, on the CTA-pair tensor-core kernel (``csrc/kernels/linear_ce.cu``):
     the log-sum-exp is taken from the fp32 products, and the backward forms the
     logits' gradient for ``piece`` vocabulary rows at a time (default: a buffer of
-    about 256 MB).  As in any matrix product, an ``inf`` or NaN in a row of ``h``
+    at most 256 MB, or 1024 rows).  As in any matrix product, an ``inf`` or NaN in a row of ``h``
     that does not count still reaches ``dw`` (0 * inf)."""
     if reduction not in _REDUCTIONS:
         raise ValueError(f"piecewise_linear_cross_entropy: reduction must be one of {sorted(_REDUCTIONS)}, "
@@ -212,14 +184,9 @@ def piecewise_linear_cross_entropy(h: torch.Tensor, w: torch.Tensor, targets: to
                         f"{h.dtype} and {w.dtype} (linear_cross_entropy takes other types)")
     if d % 8:
         raise ValueError(f"piecewise_linear_cross_entropy: d must be a multiple of 8 on CUDA, got {d}")
-    piece = _vocab_piece(rows, V) if piece is None else (int(piece) + 7) // 8 * 8
-    h2, w = _rows(h2), _rows(w)
+    piece = 0 if piece is None else (int(piece) + 7) // 8 * 8
     code = _REDUCTIONS[reduction]
-    if torch.is_grad_enabled() and (h2.requires_grad or w.requires_grad):
-        loss = _PiecewiseLinearCEFn.apply(h2, w, t.contiguous(), int(ignore_index), code, piece)
-    else:
-        losses, _, out = native().linear_ce_fwd(h2, w, t.contiguous(), int(ignore_index), code)
-        loss = losses if code == 0 else out[0]
+    loss = native().piecewise_linear_ce(_rows(h2), _rows(w), t.contiguous(), int(ignore_index), code, piece)
     return loss.view(lead) if code == 0 else loss
 
 

@@ -125,16 +125,6 @@ def test_refusals():
         ops.piecewise_linear_cross_entropy(h, w, t, piece=0)
 
 
-def test_default_piece():
-    from llm_research_b200.ops.loss import _vocab_piece
-
-    for n in (0, 1, 777, 16384, 10 ** 6):
-        for V in (1, 511, 32000, 100287):
-            p = _vocab_piece(n, V)
-            assert p % 256 == 0 and p >= 256 and -(-V // p) == -(-V // max(p, 1))
-            assert n * p * 2 <= (256 << 20) + n * 512 or p <= 1024
-
-
 # ------------------------------------------------------------------ GPU
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])

@@ -1,0 +1,202 @@
+"""The vocabulary operators as they are used together: one training step from token
+ids to the loss over a tied table (lookup, head loss in pieces, distillation), and
+HLRT's loss in pieces.
+
+The run is compared with the same step in 64 bits on the same 16-bit values.  Each
+16-bit tensor on the way (embeddings, hidden states, logits, and every gradient)
+adds half a step, relative 2^-9 for bf16, to what feeds on it; no path crosses more
+than six of them, and independent roundings of many summands do not add up beyond
+their largest, so 6 * 2^-9 of the 2-norm bounds each gradient."""
+
+import pytest
+import torch
+
+
+def _step(ids, w, mix, targets, teacher, tids, embed, ce, kd):
+    x = embed(ids, w)
+    h = torch.tanh(x @ mix)
+    logits = h @ w.t()
+    return ce(h, w, targets) + 0.5 * kd(logits, teacher, tids)
+
+
+def _plain_ce(h, w, t):
+    return torch.nn.functional.cross_entropy(h @ w.t(), t, ignore_index=-100)
+
+
+def _plain_kd(x, teacher, ids, T=2.0):
+    kept = ids >= 0
+    some = kept.any(1)
+    y = (teacher / T).masked_fill(~kept, -float("inf"))
+    y = torch.where(some[:, None], y, torch.zeros_like(y))
+    p = torch.softmax(y, 1) * kept
+    q = torch.log_softmax(x / T, 1).gather(1, ids.clamp(min=0))
+    return T * T * (torch.special.xlogy(p, p) - p * q).masked_fill(~kept, 0).sum() / some.sum()
+
+
+def _inputs(device, dtype, N=96, V=1003, d=64, K=7):
+    g = torch.Generator().manual_seed(3)
+    w = (0.3 * torch.randn(V, d, generator=g)).to(dtype)
+    mix = (torch.randn(d, d, generator=g) / 8).to(dtype)
+    ids = torch.randint(0, V, (N,), generator=g)
+    ids[::5] = 17
+    targets = torch.randint(0, V, (N,), generator=g)
+    targets[::9] = -100
+    tids = torch.stack([torch.randperm(V, generator=g)[:K] for _ in range(N)])
+    tids[3] = -1
+    tids[5, 4:] = -1
+    teacher = torch.randn(N, K, generator=g).to(dtype)
+    return [t.to(device) for t in (ids, w, mix, targets, teacher, tids)]
+
+
+def _grads(f, w, mix):
+    w, mix = w.detach().clone().requires_grad_(), mix.detach().clone().requires_grad_()
+    loss = f(w, mix)
+    return (loss.detach(), *torch.autograd.grad(loss, (w, mix)))
+
+
+def _both(device, dtype):
+    from llm_research_b200 import ops
+
+    ids, w, mix, targets, teacher, tids = _inputs(device, dtype)
+    got = _grads(lambda a, b: _step(ids, a, b, targets, teacher, tids,
+                                    lambda i, t: ops.embedding(i, t, scale=8.0),
+                                    ops.piecewise_linear_cross_entropy,
+                                    lambda x, t, i: ops.topk_distillation(x, t, i, 2.0)), w, mix)
+    ref = _grads(lambda a, b: _step(ids, a, b, targets, teacher.double(), tids, lambda i, t: 8.0 * t[i],
+                                    _plain_ce, _plain_kd), w.double(), mix.double())
+    return got, ref
+
+
+def test_step_cpu():
+    got, ref = _both("cpu", torch.float64)
+    for a, b in zip(got, ref):
+        torch.testing.assert_close(a, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_step_gpu(dtype):
+    got, ref = _both("cuda", dtype)
+    tol = 6 * torch.finfo(dtype).eps / 2
+    for a, b in zip(got, ref):
+        assert (a.double() - b).norm() <= tol * b.norm()
+    for a, b in zip(got, _both("cuda", dtype)[0]):  # the three operators are deterministic
+        assert (a.double() - b.double()).norm() <= tol * b.double().norm()
+
+
+@pytest.mark.gpu
+def test_step_captured_and_replayed():
+    """A whole step in a graph; replayed on other tokens it gives what the eager step gives."""
+    from llm_research_b200 import ops
+
+    ids, w, mix, targets, teacher, tids = _inputs("cuda", torch.bfloat16)
+    w.requires_grad_()
+
+    def step():
+        x = ops.embedding(ids, w, scale=8.0)
+        h = torch.tanh(x)
+        loss = ops.piecewise_linear_cross_entropy(h, w, targets) + ops.topk_distillation(h @ w.t(), teacher, tids, 2.0)
+        dw, = torch.autograd.grad(loss, w)
+        return loss.detach(), dw
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for shift in (0, 5):
+        ids.copy_(ids.roll(shift))
+        targets.copy_(targets.roll(shift))
+        graph.replay()
+        want = step()
+        torch.testing.assert_close(out[0], want[0])
+        torch.testing.assert_close(out[1].float(), want[1].float(), rtol=2 ** -7, atol=1e-6)
+
+
+@pytest.mark.gpu
+def test_gradients_of_these_gradients():
+    """The lookup can be differentiated twice, the two losses say that they cannot."""
+    from llm_research_b200 import ops
+
+    ids, w, mix, targets, teacher, tids = _inputs("cuda", torch.float16)
+    h = (0.1 * torch.randn(96, 64, device="cuda")).half().requires_grad_()
+    for loss in (ops.piecewise_linear_cross_entropy(h, w, targets),
+                 ops.topk_distillation(h @ w.t(), teacher, tids)):
+        dh, = torch.autograd.grad(loss, h, create_graph=True)
+        with pytest.raises(RuntimeError, match="differentiable once"):
+            (loss.sum() + dh.float().square().sum()).backward()
+
+
+def test_hlrt_loss_in_pieces():
+    from genesis.model.hlrt import HLRT
+    from genesis.training.train_phase1_bootstrap import ntp_objective
+    from llm_research_b200.models.presets import build_hlrt_config
+
+    cfg = build_hlrt_config("toy")
+    ids = torch.randint(0, cfg.vocab_size, (2, 48), generator=torch.Generator().manual_seed(1))
+    res = []
+    for how in (True, "pieces"):
+        torch.manual_seed(0)
+        m = HLRT(cfg)
+        loss = ntp_objective({"hlrt": m}, None, {"input_ids": ids, "fused_lm_loss": how})
+        loss.backward()
+        res.append((loss.detach(), {n: p.grad for n, p in m.named_parameters() if p.grad is not None}))
+    torch.testing.assert_close(res[0][0], res[1][0])
+    for n, g in res[0][1].items():
+        torch.testing.assert_close(res[1][1][n], g, atol=1e-5, rtol=1e-4, msg=n)
+    m.eval()
+    with torch.no_grad():
+        labels = torch.cat([ids[:, 1:], torch.full((2, 1), -100)], 1)
+        rows = m(ids, labels=labels, lm_loss="pieces", lm_reduction="none")["lm_loss"]
+        logits = m(ids)["logits"]
+    ref = torch.nn.functional.cross_entropy(logits.flatten(0, 1), labels.flatten(), reduction="none").view(2, 48)
+    assert rows.shape == (2, 48)
+    torch.testing.assert_close(rows, ref)
+    with pytest.raises(ValueError, match="lm_loss"):
+        m(ids, labels=labels, lm_loss="columns")
+    with pytest.raises(ValueError, match="lm_reduction"):
+        m(ids, labels=labels, lm_reduction="none")
+
+
+@pytest.mark.gpu
+def test_hlrt_trains_on_the_loss_in_pieces():
+    """bf16 HLRT on the GPU: the piecewise loss against the row-chunked one (whose logits
+    are rounded to bf16, relative 2^-9 of values below 8 here)."""
+    from genesis.model.hlrt import HLRT
+    from llm_research_b200.models.presets import build_hlrt_config
+
+    cfg = build_hlrt_config("toy")
+    torch.manual_seed(0)
+    m = HLRT(cfg).to("cuda", torch.bfloat16)
+    ids = torch.randint(0, cfg.vocab_size, (2, 64), device="cuda", generator=torch.Generator("cuda").manual_seed(1))
+    labels = torch.cat([ids[:, 1:], ids.new_full((2, 1), -100)], 1)
+    grads, losses = [], []
+    for how in ("rows", "pieces"):
+        m.zero_grad(set_to_none=True)
+        out = m(ids, labels=labels, lm_loss=how)
+        out["lm_loss"].backward()
+        losses.append(float(out["lm_loss"].detach()))
+        grads.append(m.embeddings.weight.grad.float())
+    assert abs(losses[0] - losses[1]) <= 8 * 2 ** -9
+    assert (grads[0] - grads[1]).norm() <= 0.05 * grads[0].norm()
+    assert torch.isfinite(grads[1]).all()
+
+
+@pytest.mark.gpu
+def test_verifier_distillation_from_a_stored_list():
+    from genesis.verifier.distillation import VerificationDistillation
+
+    d = VerificationDistillation(8, 4).cuda()
+    g = torch.Generator("cuda").manual_seed(4)
+    student = torch.randn(3, 5, 300, device="cuda", generator=g).requires_grad_()
+    teacher = torch.randn(3, 5, 300, device="cuda", generator=g)
+    top, ids = teacher.topk(300, dim=-1)  # the whole vocabulary: the full-vocabulary loss
+    full = d.temperature_scaled_loss(student.reshape(-1, 300), teacher.reshape(-1, 300), 2.0)
+    loss = d.topk_loss(student, top, ids, 2.0)
+    torch.testing.assert_close(loss, full, rtol=1e-5, atol=1e-6)
+    a, b = torch.autograd.grad(loss, student)[0], torch.autograd.grad(full, student)[0]
+    torch.testing.assert_close(a, b, rtol=1e-4, atol=1e-7)
