@@ -137,22 +137,55 @@ bool tracked(const at::Tensor& t) { return at::GradMode::is_enabled() && t.requi
 
 }  // namespace
 
+// `ids` of any shape and strides; out (*ids.shape, d).
 at::Tensor embedding(const at::Tensor& ids, const at::Tensor& w, double scale, int64_t padding) {
-  return tracked(w) ? EmbeddingFn::apply(w, ids, scale, padding) : embedding_fwd(ids, w, scale);
+  const at::Tensor flat = (ids.dim() == 1 ? ids : ids.reshape({-1})).contiguous();
+  const at::Tensor table = unit_columns(w);
+  const at::Tensor out =
+      tracked(table) ? EmbeddingFn::apply(table, flat, scale, padding) : embedding_fwd(flat, table, scale);
+  if (ids.dim() == 1) return out;
+  auto shape = ids.sizes().vec();
+  shape.push_back(w.size(1));
+  return out.view(shape);
 }
 
+// h (..., d), targets of its leading shape; a row loss for each target with reduction 0.
 at::Tensor piecewise_linear_ce(const at::Tensor& h, const at::Tensor& w, const at::Tensor& targets, int64_t ignore,
                                int64_t reduction, int64_t piece) {
-  if (tracked(h) || tracked(w)) return LinearCEFn::apply(h, w, targets, ignore, reduction, piece);
-  auto [rows, stats, out] = linear_ce_fwd(h, w, targets, ignore, reduction);
-  return reduction == 0 ? rows : out.select(0, 0);
+  const auto rows16 = [](const at::Tensor& t) {  // rows that the tensor maps take: 16-byte aligned, unit columns
+    return t.stride(1) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 &&
+                   t.stride(0) * (int64_t)t.element_size() % 16 == 0 && (t.stride(0) >= t.size(1) || t.size(0) <= 1)
+               ? t
+               : t.contiguous();
+  };
+  const at::Tensor h2 = rows16(h.dim() == 2 ? h : h.reshape({targets.numel(), w.size(1)})), w2 = rows16(w),
+                   t = (targets.dim() == 1 ? targets : targets.reshape({-1})).contiguous();
+  at::Tensor loss;
+  if (tracked(h2) || tracked(w2)) {
+    loss = LinearCEFn::apply(h2, w2, t, ignore, reduction, piece);
+  } else {
+    auto [rows, stats, out] = linear_ce_fwd(h2, w2, t, ignore, reduction);
+    loss = reduction == 0 ? rows : out.select(0, 0);
+  }
+  return reduction == 0 && targets.dim() != 1 ? loss.view(targets.sizes()) : loss;
 }
 
+// x (..., V); teacher and ids (..., K).  (B, S, V) views with any strides of the leading
+// dimensions are read in place.
 at::Tensor topk_distillation(const at::Tensor& x, const at::Tensor& teacher, const at::Tensor& ids, double temperature,
                              int64_t reduction) {
-  if (tracked(x)) return DistillFn::apply(x, teacher, ids, temperature, reduction);
-  auto [rows, stats, probs, out] = distill_fwd(x, teacher, ids, temperature, reduction, false);
-  return reduction == 0 ? rows : out.select(0, 0);
+  const int64_t V = x.size(-1), K = ids.size(-1);
+  const at::Tensor x3 = unit_columns(x.dim() == 3 ? x : x.dim() == 2 ? x.unsqueeze(0) : x.reshape({1, -1, V}));
+  const at::Tensor t2 = (teacher.dim() == 2 ? teacher : teacher.reshape({-1, K})).detach().contiguous(),
+                   i2 = (ids.dim() == 2 ? ids : ids.reshape({-1, K})).contiguous();
+  at::Tensor loss;
+  if (tracked(x3)) {
+    loss = DistillFn::apply(x3, t2, i2, temperature, reduction);
+  } else {
+    auto [rows, stats, probs, out] = distill_fwd(x3, t2, i2, temperature, reduction, false);
+    loss = reduction == 0 ? rows : out.select(0, 0);
+  }
+  return reduction == 0 && x.dim() != 2 ? loss.view(x.sizes().slice(0, x.dim() - 1)) : loss;
 }
 
 }  // namespace lrb

@@ -69,18 +69,12 @@ def topk_distillation(logits: torch.Tensor, teacher_logits: torch.Tensor, teache
     if V < 1 or K < 1 or teacher_logits.shape != teacher_ids.shape or teacher_ids.shape[:-1] != lead:
         raise ValueError(f"topk_distillation: logits (..., V) and teacher (..., K) with one leading shape, got "
                          f"{tuple(logits.shape)}, {tuple(teacher_logits.shape)}, {tuple(teacher_ids.shape)}")
-    teacher, ids = teacher_logits.detach().reshape(-1, K), teacher_ids.reshape(-1, K)
     if not logits.is_cuda:
-        rows = _plain(logits.reshape(-1, V), teacher, ids, T, reduction)
+        rows = _plain(logits.reshape(-1, V), teacher_logits.reshape(-1, K), teacher_ids.reshape(-1, K), T, reduction)
         return rows.reshape(lead) if reduction == "none" else rows
     if K > MAX_TEACHER_ENTRIES:
         raise ValueError(f"topk_distillation: at most {MAX_TEACHER_ENTRIES} teacher entries on CUDA, got {K}")
-    for name, t in (("logits", logits), ("teacher_logits", teacher)):
+    for name, t in (("logits", logits), ("teacher_logits", teacher_logits)):
         if t.dtype not in _DTYPES:
             raise TypeError(f"topk_distillation: {name} must be bf16, fp16 or fp32 on CUDA, got {t.dtype}")
-    # (B, S, V) views with any strides of the leading dimensions (logits[:, :-1]) are read in place
-    x = logits if logits.dim() == 3 else logits.unsqueeze(0) if logits.dim() == 2 else logits.reshape(1, -1, V)
-    if x.stride(-1) != 1 and V > 1:
-        x = x.contiguous()
-    out = native().topk_distillation(x, teacher.contiguous(), ids.contiguous(), T, _REDUCTIONS[reduction])
-    return out.view(lead) if reduction == "none" else out
+    return native().topk_distillation(logits, teacher_logits, teacher_ids, T, _REDUCTIONS[reduction])

@@ -44,10 +44,4 @@ def embedding(ids: torch.Tensor, weight: torch.Tensor, scale: float = 1.0,
         return out * scale if out.dtype in (torch.float32, torch.float64) else (out.float() * scale).to(out.dtype)
     if weight.dtype not in _DTYPES:
         raise TypeError(f"embedding: weight must be bf16, fp16 or fp32 on CUDA, got {weight.dtype}")
-    flat = ids.reshape(-1)
-    if not flat.is_contiguous():
-        flat = flat.contiguous()
-    if weight.stride(1) != 1:
-        weight = weight.contiguous()
-    out = native().embedding(flat, weight, scale, -1 if padding_idx is None else padding_idx)
-    return out.view(*ids.shape, weight.shape[1])
+    return native().embedding(ids, weight, scale, -1 if padding_idx is None else padding_idx)

@@ -168,16 +168,15 @@ def piecewise_linear_cross_entropy(h: torch.Tensor, w: torch.Tensor, targets: to
     if piece is not None and piece < 1:
         raise ValueError(f"piecewise_linear_cross_entropy: piece must be positive, got {piece}")
     V, d = w.shape
-    lead, rows = targets.shape, targets.numel()
-    h2, t = h.reshape(rows, d), targets.reshape(rows)
     if not h.is_cuda:
+        h2, t = h.reshape(targets.numel(), d), targets.reshape(-1)
         f = torch.float64 if h.dtype == torch.float64 else torch.float32
         counted = (t != ignore_index) & (t >= 0) & (t < V)
         logq = torch.log_softmax(F.linear(h2.to(f), w.to(f)), dim=-1)
         loss = -logq.gather(1, t.clamp(0, V - 1)[:, None]).squeeze(1)
         loss = torch.where(counted, loss, torch.zeros_like(loss))
         if reduction == "none":
-            return loss.reshape(lead)
+            return loss.reshape(targets.shape)
         return loss.sum() if reduction == "sum" else loss.sum() / counted.sum().clamp(min=1)
     if h.dtype not in (torch.bfloat16, torch.float16) or w.dtype != h.dtype:
         raise TypeError(f"piecewise_linear_cross_entropy: h and w must both be bf16 or both fp16 on CUDA, got "
@@ -185,9 +184,7 @@ def piecewise_linear_cross_entropy(h: torch.Tensor, w: torch.Tensor, targets: to
     if d % 8:
         raise ValueError(f"piecewise_linear_cross_entropy: d must be a multiple of 8 on CUDA, got {d}")
     piece = 0 if piece is None else (int(piece) + 7) // 8 * 8
-    code = _REDUCTIONS[reduction]
-    loss = native().piecewise_linear_ce(_rows(h2), _rows(w), t.contiguous(), int(ignore_index), code, piece)
-    return loss.view(lead) if code == 0 else loss
+    return native().piecewise_linear_ce(h, w, targets, int(ignore_index), _REDUCTIONS[reduction], piece)
 
 
 # ------------------------------------------------ vocabulary-parallel linear + CE
