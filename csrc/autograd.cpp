@@ -12,13 +12,15 @@ namespace lrb {
 
 at::Tensor embedding_fwd(const at::Tensor&, const at::Tensor&, double);
 at::Tensor embedding_bwd(const at::Tensor&, const at::Tensor&, int64_t, int64_t, double);
-std::tuple<at::Tensor, at::Tensor, at::Tensor> linear_ce_fwd(const at::Tensor&, const at::Tensor&, const at::Tensor&,
-                                                             int64_t, int64_t);
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> linear_ce_fwd(const at::Tensor&, const at::Tensor&,
+                                                                         const at::Tensor&, int64_t, int64_t);
 std::tuple<at::Tensor, at::Tensor> linear_ce_bwd(const at::Tensor&, const at::Tensor&, const at::Tensor&, int64_t,
                                                  const at::Tensor&, const at::Tensor&, bool, const at::Tensor&, int64_t,
                                                  bool, bool);
-std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> distill_fwd(const at::Tensor&, const at::Tensor&,
-                                                                       const at::Tensor&, double, int64_t, bool);
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> distill_fwd(const at::Tensor&,
+                                                                                   const at::Tensor&,
+                                                                                   const at::Tensor&, double, int64_t,
+                                                                                   bool);
 at::Tensor distill_bwd(const at::Tensor&, const at::Tensor&, double, const at::Tensor&, const at::Tensor&,
                        const at::Tensor&, bool, const at::Tensor&);
 
@@ -87,12 +89,12 @@ variable_list EmbeddingFn::backward(AutogradContext* ctx, variable_list g) {
 struct LinearCEFn : public Function<LinearCEFn> {
   static Variable forward(AutogradContext* ctx, const Variable& h, const Variable& w, const Variable& targets,
                           int64_t ignore, int64_t reduction, int64_t piece) {
-    auto [rows, stats, out] = linear_ce_fwd(h, w, targets, ignore, reduction);
-    ctx->save_for_backward({h, w, targets, stats, out});
+    auto [rows, stats, out, factor] = linear_ce_fwd(h, w, targets, ignore, reduction);
+    ctx->save_for_backward({h, w, targets, stats, factor});
     ctx->saved_data["ignore"] = ignore;
     ctx->saved_data["per_row"] = reduction == 0;
     ctx->saved_data["piece"] = piece;
-    return reduction == 0 ? rows : out.select(0, 0);
+    return reduction == 0 ? rows : out;
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     const auto s = ctx->get_saved_variables();
@@ -103,7 +105,7 @@ struct LinearCEFn : public Function<LinearCEFn> {
       at::AutoGradMode off(false);
       std::tie(dh, dw) = linear_ce_bwd(s[0], s[1], s[2], ctx->saved_data["ignore"].toInt(), s[3],
                                        g[0].to(at::kFloat).contiguous(), per_row,
-                                       per_row ? s[3] : s[4].narrow(0, 1, 1), ctx->saved_data["piece"].toInt(), need_h,
+                                       per_row ? s[3] : s[4], ctx->saved_data["piece"].toInt(), need_h,
                                        need_w);
     }
     return once("piecewise_linear_cross_entropy", {need_h ? dh : Variable(), need_w ? dw : Variable(), Variable(),
@@ -114,11 +116,11 @@ struct LinearCEFn : public Function<LinearCEFn> {
 struct DistillFn : public Function<DistillFn> {
   static Variable forward(AutogradContext* ctx, const Variable& x, const Variable& teacher, const Variable& ids,
                           double temperature, int64_t reduction) {
-    auto [rows, stats, probs, out] = distill_fwd(x, teacher, ids, temperature, reduction, true);
-    ctx->save_for_backward({x, ids, stats, probs, out});
+    auto [rows, stats, probs, out, factor] = distill_fwd(x, teacher, ids, temperature, reduction, true);
+    ctx->save_for_backward({x, ids, stats, probs, factor});
     ctx->saved_data["temperature"] = temperature;
     ctx->saved_data["per_row"] = reduction == 0;
-    return reduction == 0 ? rows : out.select(0, 0);
+    return reduction == 0 ? rows : out;
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     const auto s = ctx->get_saved_variables();
@@ -127,7 +129,7 @@ struct DistillFn : public Function<DistillFn> {
     {
       at::AutoGradMode off(false);
       dx = distill_bwd(s[0], s[1], ctx->saved_data["temperature"].toDouble(), s[2], s[3],
-                       g[0].to(at::kFloat).contiguous(), per_row, per_row ? s[2] : s[4].narrow(0, 1, 1));
+                       g[0].to(at::kFloat).contiguous(), per_row, per_row ? s[2] : s[4]);
     }
     return once("topk_distillation", {dx, Variable(), Variable(), Variable(), Variable()});
   }
@@ -164,8 +166,8 @@ at::Tensor piecewise_linear_ce(const at::Tensor& h, const at::Tensor& w, const a
   if (tracked(h2) || tracked(w2)) {
     loss = LinearCEFn::apply(h2, w2, t, ignore, reduction, piece);
   } else {
-    auto [rows, stats, out] = linear_ce_fwd(h2, w2, t, ignore, reduction);
-    loss = reduction == 0 ? rows : out.select(0, 0);
+    auto [rows, stats, out, factor] = linear_ce_fwd(h2, w2, t, ignore, reduction);
+    loss = reduction == 0 ? rows : out;
   }
   return reduction == 0 && targets.dim() != 1 ? loss.view(targets.sizes()) : loss;
 }
@@ -182,8 +184,8 @@ at::Tensor topk_distillation(const at::Tensor& x, const at::Tensor& teacher, con
   if (tracked(x3)) {
     loss = DistillFn::apply(x3, t2, i2, temperature, reduction);
   } else {
-    auto [rows, stats, probs, out] = distill_fwd(x3, t2, i2, temperature, reduction, false);
-    loss = reduction == 0 ? rows : out.select(0, 0);
+    auto [rows, stats, probs, out, factor] = distill_fwd(x3, t2, i2, temperature, reduction, false);
+    loss = reduction == 0 ? rows : out;
   }
   return reduction == 0 && x.dim() != 2 ? loss.view(x.sizes().slice(0, x.dim() - 1)) : loss;
 }

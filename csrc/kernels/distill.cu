@@ -389,11 +389,11 @@ __global__ void __launch_bounds__(kThreads, (kFwdBlocks<T, W>))
   }
 }
 
-// out[0] = the loss (sum of the rows, over the number of counted rows for a mean),
-// out[1] = each counted row's factor in it.  One block, fixed order.
+// The loss (sum of the rows, over the number of counted rows for a mean) and each
+// counted row's factor in it.  One block, fixed order.
 __global__ void __launch_bounds__(1024) reduce_rows_kernel(const float* __restrict__ loss,
                                                            const float* __restrict__ counted, int64_t n, int mean,
-                                                           float* __restrict__ out) {
+                                                           float* __restrict__ out, float* __restrict__ factor) {
   __shared__ double rs[32], rc[32];
   double s = 0.0, c = 0.0;
   for (int64_t i = threadIdx.x; i < n; i += 1024) {
@@ -417,8 +417,8 @@ __global__ void __launch_bounds__(1024) reduce_rows_kernel(const float* __restri
       c += rc[w];
     }
     const double f = mean ? 1.0 / (c > 1.0 ? c : 1.0) : 1.0;
-    out[0] = (float)(s * f);
-    out[1] = (float)f;
+    *out = (float)(s * f);
+    *factor = (float)f;
   }
 }
 
@@ -600,12 +600,12 @@ bool warp_a_row(int64_t n, int64_t row_bytes, int K, int64_t most) {
 
 // logits (outer, inner, V); teacher (outer * inner, K).  Returns (row losses, row
 // statistics (N, 4) and the teacher's probabilities (N, K) for the backward -- the
-// latter left empty without `keep` --, [loss, factor]); the last is filled for a sum or
-// a mean (reduction 1, 2) and left empty for 0.
-std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> distill_fwd(const at::Tensor& logits,
-                                                                       const at::Tensor& t_logits,
-                                                                       const at::Tensor& t_ids, double temperature,
-                                                                       int64_t reduction, bool keep) {
+// latter left empty without `keep` --, the loss and each counted row's factor in it (of
+// a sum or a mean, reduction 1 and 2; not filled for 0)).  The loss is a tensor of its
+// own: a caller may change it in place.
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> distill_fwd(
+    const at::Tensor& logits, const at::Tensor& t_logits, const at::Tensor& t_ids, double temperature,
+    int64_t reduction, bool keep) {
   const Rows rows = make_rows(logits, "topk_distillation");
   const int64_t n = logits.size(0) * logits.size(1), V = logits.size(2);
   const Teacher t = make_teacher(t_logits, t_ids, logits, n, "topk_distillation");
@@ -613,8 +613,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> distill_fwd(const at:
   c10::cuda::CUDAGuard g(logits.device());
   bind_device(logits.get_device());
   auto f32 = logits.options().dtype(at::kFloat);
-  auto loss = at::empty({n}, f32), rest = at::empty({5 * n + (reduction == 0 ? 0 : 2)}, f32);
-  auto stats = rest.narrow(0, 0, 4 * n), out = rest.narrow(0, 5 * n, reduction == 0 ? 0 : 2);
+  auto loss = at::empty({n}, f32), rest = at::empty({5 * n + 1}, f32), out = at::empty({}, f32);
+  auto stats = rest.narrow(0, 0, 4 * n), factor = rest.narrow(0, 5 * n, 1);
   float* counted = rest.data_ptr<float>() + 4 * n;
   auto probs = at::empty({keep ? n : 0, t.K}, f32);
   if (n > 0) {
@@ -641,10 +641,10 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> distill_fwd(const at:
   }
   if (reduction != 0) {
     reduce_rows_kernel<<<1, 1024, 0, stream()>>>(loss.data_ptr<float>(), counted, n, reduction == 2 ? 1 : 0,
-                                                 out.data_ptr<float>());
+                                                 out.data_ptr<float>(), factor.data_ptr<float>());
     LRB_LAUNCH_CHECK();
   }
-  return {loss, stats, probs, out};
+  return {loss, stats, probs, out, factor};
 }
 
 // Gradient of the logits (contiguous, their shape): `g` fp32, one value for each row
@@ -677,8 +677,9 @@ at::Tensor distill_bwd(const at::Tensor& logits, const at::Tensor& t_ids, double
 }
 
 // The same reduction for other per-row losses (reduction 1: sum, 2: mean over the counted rows).
-void reduce_rows(const float* loss, const float* counted, int64_t n, bool mean, float* out, cudaStream_t s) {
-  reduce_rows_kernel<<<1, 1024, 0, s>>>(loss, counted, n, mean ? 1 : 0, out);
+void reduce_rows(const float* loss, const float* counted, int64_t n, bool mean, float* out, float* factor,
+                 cudaStream_t s) {
+  reduce_rows_kernel<<<1, 1024, 0, s>>>(loss, counted, n, mean ? 1 : 0, out, factor);
   LRB_LAUNCH_CHECK();
 }
 

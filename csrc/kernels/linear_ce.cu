@@ -30,7 +30,7 @@ int gemm_pair_slices(int64_t, int64_t, int64_t, int);
 int64_t gemm_pair_ce_piece(int64_t, int64_t, int64_t, int64_t, int);
 void gemm_pair_sliced(const at::Tensor&, const at::Tensor&, bool, bool, at::Tensor&, int, bool, const float*);
 // distill.cu
-void reduce_rows(const float*, const float*, int64_t, bool, float*, cudaStream_t);
+void reduce_rows(const float*, const float*, int64_t, bool, float*, float*, cudaStream_t);
 
 namespace {
 
@@ -147,19 +147,18 @@ void check_head_inputs(const at::Tensor& h, const at::Tensor& w, const at::Tenso
 
 }  // namespace
 
-// Returns (row losses, row statistics (N, 2), [loss, factor]); the last is left empty
-// for reduction 0 (none), 1 is the sum and 2 the mean over the counted rows.
-std::tuple<at::Tensor, at::Tensor, at::Tensor> linear_ce_fwd(const at::Tensor& h, const at::Tensor& w,
-                                                             const at::Tensor& targets, int64_t ignore,
-                                                             int64_t reduction) {
+// Returns (row losses, row statistics (N, 2), the loss and each counted row's factor in
+// it: reduction 1 is the sum and 2 the mean over the counted rows; not filled for 0).
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> linear_ce_fwd(const at::Tensor& h, const at::Tensor& w,
+                                                                         const at::Tensor& targets, int64_t ignore,
+                                                                         int64_t reduction) {
   check_head_inputs(h, w, targets);
   c10::cuda::CUDAGuard guard(h.device());
   bind_device(h.get_device());
   const int64_t n = h.size(0), V = w.size(0);
   auto f32 = h.options().dtype(at::kFloat);
   auto loss = at::empty({n}, f32), stats = at::empty({n, 2}, f32);
-  auto out = at::empty({reduction == 0 ? 0 : 2}, f32);
-  auto counted = at::empty({n}, f32);
+  auto out = at::empty({}, f32), factor = at::empty({1}, f32), counted = at::empty({n}, f32);
   if (n > 0) {
     const int64_t tiles = gemm_pair_lse_tiles(V);
     auto part = at::empty({tiles, n, 2}, f32), target_logit = at::empty({n}, f32);
@@ -171,8 +170,9 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> linear_ce_fwd(const at::Tensor& h
     LRB_LAUNCH_CHECK();
   }
   if (reduction != 0)
-    reduce_rows(loss.data_ptr<float>(), counted.data_ptr<float>(), n, reduction == 2, out.data_ptr<float>(), stream());
-  return {loss, stats, out};
+    reduce_rows(loss.data_ptr<float>(), counted.data_ptr<float>(), n, reduction == 2, out.data_ptr<float>(),
+                factor.data_ptr<float>(), stream());
+  return {loss, stats, out, factor};
 }
 
 // (dh, dw), each empty where it is not asked for.  `g` fp32: one value for each row,

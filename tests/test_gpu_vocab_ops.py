@@ -200,3 +200,26 @@ def test_verifier_distillation_from_a_stored_list():
     torch.testing.assert_close(loss, full, rtol=1e-5, atol=1e-6)
     a, b = torch.autograd.grad(loss, student)[0], torch.autograd.grad(full, student)[0]
     torch.testing.assert_close(a, b, rtol=1e-4, atol=1e-7)
+
+
+@pytest.mark.gpu
+def test_losses_changed_in_place():
+    """``loss /= steps`` before the backward, as accumulation loops do."""
+    from llm_research_b200 import ops
+
+    ids, w, mix, targets, teacher, tids = _inputs("cuda", torch.bfloat16)
+    h = (0.1 * torch.randn(96, 64, device="cuda")).bfloat16().requires_grad_()
+    x = (h @ w.t()).detach().requires_grad_()
+    for leaf, f in ((h, lambda red: ops.piecewise_linear_cross_entropy(h, w, targets, reduction=red)),
+                    (x, lambda red: ops.topk_distillation(x, teacher, tids, reduction=red))):
+        for red in ("mean", "sum", "none"):
+            up = torch.ones((), device="cuda") if red != "none" else torch.ones(96, device="cuda")
+            want, = torch.autograd.grad(f(red), leaf, up / 4)
+            loss = f(red)
+            loss /= 4
+            got, = torch.autograd.grad(loss, leaf, up)
+            assert torch.equal(got, want)
+    out = ops.embedding(ids.view(8, 12), w.requires_grad_())
+    out *= 2
+    dw, = torch.autograd.grad(out.float().sum(), w)
+    assert dw[17, 0] == 2 * float((ids == 17).sum())
