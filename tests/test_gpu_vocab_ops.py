@@ -223,3 +223,57 @@ def test_losses_changed_in_place():
     out *= 2
     dw, = torch.autograd.grad(out.float().sum(), w)
     assert dw[17, 0] == 2 * float((ids == 17).sum())
+
+
+@pytest.mark.gpu
+def test_offsets_past_32_bits():
+    """Tables, hidden states and logits of more than 2^31 elements."""
+    from llm_research_b200 import ops
+
+    V, d = 1100003, 2048
+    g = torch.Generator("cuda").manual_seed(6)
+    w = torch.empty(V, d, device="cuda", dtype=torch.bfloat16)
+    for b in range(0, V, 1 << 17):
+        w[b:b + (1 << 17)] = torch.randn(min(1 << 17, V - b), d, device="cuda", generator=g) / d ** 0.5
+    w.requires_grad_()
+    ids = torch.tensor([V - 1, 0, V - 1, 1048577, 5], device="cuda")
+    out = ops.embedding(ids, w)
+    assert torch.equal(out, w[ids])
+    dy = torch.randn(5, d, device="cuda", generator=g).bfloat16()
+    dw, = torch.autograd.grad(out, w, dy)
+    assert torch.equal(dw[[0, 1048577, 5]], dy[[1, 3, 4]])
+    assert torch.equal(dw[V - 1], (dy[0].float() + dy[2].float()).bfloat16())
+    assert dw[6:1048577].any().item() is False and dw[1048578:V - 1].any().item() is False
+    del dw
+
+    h = torch.randn(4, d, device="cuda", generator=g).bfloat16().requires_grad_()
+    t = torch.tensor([V - 1, 1, 1048577, -100], device="cuda")
+    loss = ops.piecewise_linear_cross_entropy(h, w, t, reduction="none")
+    z = torch.cat([h.detach().float() @ w.detach()[b:b + (1 << 17)].float().t() for b in range(0, V, 1 << 17)], 1)
+    ref = torch.nn.functional.cross_entropy(z.double(), t, reduction="none", ignore_index=-100)
+    assert (loss.double() - ref).abs().max() < 1e-4
+    dh, dw = torch.autograd.grad(loss, (h, w), torch.ones(4, device="cuda"))
+    p = torch.softmax(z.double(), 1)
+    for j in (0, 1, 1048577, V - 2, V - 1):
+        dz = (p[:, j] - (t == j).double()) * (t >= 0)
+        row = dz @ h.detach().double()
+        # dz and the result are rounded once each (2^-9), fp32 sums in between
+        assert (dw[j].double() - row).abs().max() <= 2 ** -8 * 1.01 * (dz.abs()[:, None] * h.detach().double().abs()).sum(0).max()
+    assert dh[3].eq(0).all()
+    del dh, dw, w, z, p
+
+    n, V = 70001, 32001
+    x = torch.zeros(n, V, device="cuda", dtype=torch.bfloat16)
+    x[-2:] = torch.randn(2, V, device="cuda", generator=g)
+    tids = torch.full((n, 3), -1, device="cuda")
+    tids[-2:] = torch.tensor([[7, V - 1, 2], [V - 2, 0, 1]], device="cuda")
+    teacher = torch.randn(n, 3, device="cuda", generator=g)
+    x.requires_grad_()
+    rows = ops.topk_distillation(x, teacher, tids, reduction="none")
+    dx, = torch.autograd.grad(rows, x, torch.ones(n, device="cuda"))
+    tail = x.detach()[-2:].double().requires_grad_()
+    want = _plain_kd(tail, teacher[-2:].double(), tids[-2:], 1.0) * 2
+    torch.testing.assert_close(rows[-2:].sum().double(), want.detach(), rtol=1e-5, atol=1e-5)
+    ref, = torch.autograd.grad(want, tail)
+    assert (dx[-2:].double() - ref).abs().max() <= 2 ** -9 * ref.abs().max() + 1e-6
+    assert rows[:-2].eq(0).all() and not dx[:-2].any()
