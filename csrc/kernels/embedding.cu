@@ -554,24 +554,25 @@ at::Tensor embedding_bwd(const at::Tensor& dy, const at::Tensor& ids, int64_t V,
   });
   const int64_t ranges = (n + a.range - 1) / a.range;
   // at most one token crosses each border
-  auto buf = at::empty({4 * ranges + 4 + 6 * n}, ids.options().dtype(at::kInt));
+  const bool join = ranges > 1;
+  const int64_t ints = (4 * ranges + 4 + 6 * n + 3) / 4 * 4;
+  auto buf = at::empty({ints + (join ? 2 * ranges * d : 0)}, ids.options().dtype(at::kInt));
   int* p = buf.data_ptr<int>();
   int4* spans = reinterpret_cast<int4*>(p);
+  float* partial = reinterpret_cast<float*>(p + ints);
   a.num_spans = p + 4 * ranges;
   a.pair_a = reinterpret_cast<int2*>(a.num_spans + 4), a.pair_b = a.pair_a + n;
   a.key = a.num_spans + 4 + 4 * n, a.pos = a.key + n;
-  const bool join = ranges > 1;
-  auto partial = at::empty({join ? 2 * ranges * d : 0}, dy.options().dtype(at::kFloat));
   if (ids.scalar_type() == at::kLong) launch_sort<int64_t>(ids, a, blocks);
   else launch_sort<int>(ids, a, blocks);
   launch_fill(dw);
   LRB_DISPATCH_FLOAT(dy.scalar_type(), T, [&] {
-    if (vec) launch_sum<T, 16 / sizeof(T)>(dy, a, partial.data_ptr<float>(), spans, dw, (int)d, scale);
-    else launch_sum<T, 1>(dy, a, partial.data_ptr<float>(), spans, dw, (int)d, scale);
+    if (vec) launch_sum<T, 16 / sizeof(T)>(dy, a, partial, spans, dw, (int)d, scale);
+    else launch_sum<T, 1>(dy, a, partial, spans, dw, (int)d, scale);
     if (join) {
       const int slices = (int)((d + 127) / 128);
       embedding_join_kernel<T><<<(unsigned)std::min<int64_t>((ranges * slices + 7) / 8, (int64_t)num_sms() * 8), 256, 0,
-                                 stream()>>>(spans, a.num_spans, (int)ranges, partial.data_ptr<float>(),
+                                 stream()>>>(spans, a.num_spans, (int)ranges, partial,
                                              reinterpret_cast<T*>(dw.data_ptr()), (int)d, slices, (float)scale);
       LRB_LAUNCH_CHECK();
     }

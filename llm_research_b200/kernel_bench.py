@@ -24,6 +24,10 @@ Cases (shapes are the GENESIS-1B / 7B working shapes):
   swiglu_fwd             32768 x (2 x 5632) bf16
   ns                     Newton-Schulz, 5 iterations, batch 8 of 2048 x 5632
   ce                     cross-entropy fwd+bwd, 32768 x 32000 bf16 logits
+  embedding              token lookup fwd + gradient, 65536 tokens of 32000 x 2048 bf16
+  linear_ce_pieces       head + cross-entropy in pieces of the vocabulary, fwd+bwd,
+                         16384 x 32000 x 2048 bf16 (8 N V d operations: the logits are formed twice)
+  distill                top-64 distillation fwd+bwd, 16384 x 32000 bf16 logits
 """
 
 from __future__ import annotations
@@ -190,6 +194,33 @@ def _cases() -> Dict[str, Callable[[], Tuple[Callable[[], None], float, float]]]
 
         return run, 0.0, logits.numel() * 2 * 3.0
 
+    def embedding():
+        from llm_research_b200 import ops
+
+        T, V, d = 65536, 32000, 2048
+        ids = torch.randint(0, V, (T,), device="cuda")
+        w = torch.randn(V, d, device="cuda", dtype=torch.bfloat16).requires_grad_()
+        dy = torch.randn(T, d, device="cuda", dtype=torch.bfloat16)
+        return (lambda: torch.autograd.grad(ops.embedding(ids, w), w, dy)), 0.0, 2.0 * (2 * T * d + 2 * V * d)
+
+    def linear_ce_pieces():
+        from llm_research_b200 import ops
+
+        T, V, d = 16384, 32000, 2048
+        h = torch.randn(T, d, device="cuda", dtype=torch.bfloat16).requires_grad_()
+        w = (torch.randn(V, d, device="cuda") * 0.02).to(torch.bfloat16).requires_grad_()
+        t = torch.randint(0, V, (T,), device="cuda")
+        return (lambda: torch.autograd.grad(ops.piecewise_linear_cross_entropy(h, w, t), (h, w))), 8.0 * T * V * d, 0.0
+
+    def distill():
+        from llm_research_b200 import ops
+
+        T, V, K = 16384, 32000, 64
+        x = torch.randn(T, V, device="cuda", dtype=torch.bfloat16).requires_grad_()
+        ids = (torch.randint(0, V, (T, 1), device="cuda") + torch.arange(K, device="cuda") * (V // K)) % V
+        teacher = torch.randn(T, K, device="cuda", dtype=torch.bfloat16)
+        return (lambda: torch.autograd.grad(ops.topk_distillation(x, teacher, ids, 2.0), x)), 0.0, 2.0 * 3 * T * V
+
     cases = {
         "attn_fwd": lambda: _attn_case(4, 4096, 16, 16, False),
         "attn_bwd": lambda: _attn_case(4, 4096, 16, 16, True),
@@ -210,6 +241,7 @@ def _cases() -> Dict[str, Callable[[], Tuple[Callable[[], None], float, float]]]
         "ce": ce,
         "gemm_pair": gemm_pair,
     }
+    cases.update(embedding=embedding, linear_ce_pieces=linear_ce_pieces, distill=distill)
     cases["lin_upgate_swiglu"] = _swiglu_up_case
     cases["lin_qkv_rope"] = _qkv_rope_case
     for name, (N, K) in LINEAR_SHAPES.items():
