@@ -16,9 +16,11 @@
 // Rows whose maximum is beyond 1e30, where x k2 - B would overflow (a row of the
 // type's lowest values), take differences x - m first.
 //
-// Bounded by the bytes of the logits; for 16-bit logits the 16 exponentials a clock
-// and SM are the next limit (12 at the copy rate), so the rest is kept short: maxima
-// of 16-bit pairs, packed fp32 fma and add.
+// Bounded by the bytes of the logits: 16384 x 32000 bf16 with 64 entries forward 196 us
+// (5.4 TB/s) and backward 320 us (6.6 TB/s), 4093 x 100287 fp32 with 200 entries 261 us
+// and 559 us (6.3 and 5.9 TB/s).  The 16-bit forward is the furthest from the copy rate
+// (6.5 TB/s): its exponentials keep the special-function pipe 71 % busy and every row
+// ends in a join; moving a quarter of the exponentials to the FMA pipe did not help.
 #include "../common.cuh"
 
 #include <cmath>
@@ -33,12 +35,13 @@ constexpr int kWarpK = kPerThread * 32;         // for a warp a row
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr float kFar = 1e30f;
 
-// Vectors in flight a thread (U) and blocks an SM, measured: 16384 x 32000 bf16 forward
-// 199 us at 8 / 4 with a warp a row and 201 to 218 us at 4 / 5 and 4 / 6 with a block a row;
-// 4093 x 100287 fp32 261 us at 8 / 4 (291 at 4 / 6).  Backward 320 us at 4 / 5 (335 at
-// 4 / 8, 338 at 8 / 4) and 559 us at 4 / any (587 at 4 / 5).
+// Vectors in flight a thread (U) and blocks an SM, measured.  Forward: 16384 x 32000 bf16
+// 196 us at 4 / 6 (212 at 4 / 5, 194 at 4 / 8; a warp a row 199 at 8 / 4), 2048 x 100287
+// bf16 80 us at 4 / 6 (79 at 4 / 5, 83 at 4 / 8); 4093 x 100287 fp32 261 us at 8 / 4 (291 at
+// 4 / 6).  Backward: 320 us at 4 / 5 (335 at 4 / 8, 338 at 8 / 4), fp32 559 us at 4 / any
+// (587 at 4 / 5).
 template <typename T, int W> constexpr int kFwdU = W == 1 || sizeof(T) == 4 ? 8 : 4;
-template <typename T, int W> constexpr int kFwdBlocks = W == 1 || sizeof(T) == 4 ? 4 : 5;
+template <typename T, int W> constexpr int kFwdBlocks = W == 1 || sizeof(T) == 4 ? 4 : 6;
 template <typename T, int W> constexpr int kBwdU = W == 1 ? 8 : 4;
 template <typename T, int W> constexpr int kBwdBlocks = W == 1 ? 4 : sizeof(T) == 4 ? 1 : 5;
 
@@ -164,17 +167,10 @@ struct Online {
   }
 };
 
-// (m, s) pairs whose s refer to the base of their own m.
-__device__ __forceinline__ float2 join(float2 a, float2 b, float k2) {
-  const float m = fmaxf(a.x, b.x);
-  const float base = base_of(m, k2);
-  return make_float2(m, a.y * fast_exp2(base_of(a.x, k2) - base) + b.y * fast_exp2(base_of(b.x, k2) - base));
-}
+// (m, s) pairs whose s refer to the base of their own m, joined over a warp.
 __device__ __forceinline__ float2 warp_join(float2 v, float k2) {
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1)
-    v = join(v, make_float2(__shfl_xor_sync(0xffffffffu, v.x, o), __shfl_xor_sync(0xffffffffu, v.y, o)), k2);
-  return v;
+  const float m = warp_max(v.x);
+  return make_float2(m, warp_sum(v.y * fast_exp2(base_of(v.x, k2) - base_of(m, k2))));
 }
 
 __device__ __forceinline__ unsigned cluster_rank() {
@@ -650,7 +646,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> distill_f
 namespace {
 // The gradient's tensor: laid out like the logits where these are a view with gaps
 // (logits[:, :-1]) of little waste, and at the same offset from a 16-byte boundary, so
-// that a row's vectors are aligned on both sides (501 columns of bf16: 4x the time when
+// that a row's vectors are aligned on both sides (4096 x 32001 bf16: 150 us both ways, 443 us when
 // they are not).  Contiguous otherwise.
 at::Tensor gradient_like(const at::Tensor& x) {
   const int64_t esz = x.element_size(), B = x.size(0), S = x.size(1), V = x.size(2), sb = x.stride(0), ss = x.stride(1);

@@ -118,6 +118,45 @@ def test_step_captured_and_replayed():
 
 
 @pytest.mark.gpu
+def test_two_streams_at_once():
+    """Calls in flight on two streams share no workspace: the results are those of one after the other."""
+    from llm_research_b200 import ops
+
+    def inputs(seed):
+        g = torch.Generator("cuda").manual_seed(seed)
+        ids = torch.randint(0, 5000, (9000,), device="cuda", generator=g)
+        w = (0.1 * torch.randn(5000, 128, device="cuda", generator=g)).bfloat16().requires_grad_()
+        h = torch.randn(700, 128, device="cuda", generator=g).bfloat16().requires_grad_()
+        x = torch.randn(700, 5000, device="cuda", generator=g).bfloat16().requires_grad_()
+        t = torch.randint(0, 5000, (700,), device="cuda", generator=g)
+        te = torch.randn(700, 20, device="cuda", generator=g)
+        ti = torch.randint(0, 5000, (700, 20), device="cuda", generator=g)
+        dy = torch.randn(9000, 128, device="cuda", generator=g).bfloat16()
+        return ids, w, h, x, t, te, ti, dy
+
+    def run(ids, w, h, x, t, te, ti, dy):
+        one = torch.ones((), device="cuda")
+        dw, = torch.autograd.grad(ops.embedding(ids, w, 2.0), w, dy)
+        ce = torch.autograd.grad(ops.piecewise_linear_cross_entropy(h, w, t, piece=1024), (h, w), one)
+        dx, = torch.autograd.grad(ops.topk_distillation(x, te, ti, 2.0), x, one)
+        return dw, *ce, dx
+
+    sets = [inputs(s) for s in (1, 2)]
+    want = [run(*s) for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    got = [None, None]
+    for _ in range(5):
+        for k, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[k] = run(*sets[k])
+    torch.cuda.synchronize()
+    for a, b in zip(want, got):
+        for u, v in zip(a, b):
+            assert torch.equal(u, v)
+
+
+@pytest.mark.gpu
 def test_gradients_of_these_gradients():
     """The lookup can be differentiated twice, the two losses say that they cannot."""
     from llm_research_b200 import ops
