@@ -16,8 +16,8 @@
 // Rows whose maximum is beyond 1e30, where x k2 - B would overflow (a row of the
 // type's lowest values), take differences x - m first.
 //
-// Bounded by the bytes of the logits: 16384 x 32000 bf16 with 64 entries forward 196 us
-// (5.4 TB/s) and backward 320 us (6.6 TB/s), 4093 x 100287 fp32 with 200 entries 261 us
+// Bounded by the bytes of the logits: 16384 x 32000 bf16 with 64 entries forward 196 to
+// 204 us (5.1 to 5.4 TB/s) and backward 317 us (6.6 TB/s), 4093 x 100287 fp32 with 200 entries 261 us
 // and 559 us (6.3 and 5.9 TB/s).  The 16-bit forward is the furthest from the copy rate
 // (6.5 TB/s): its exponentials keep the special-function pipe 71 % busy and every row
 // ends in a join; moving a quarter of the exponentials to the FMA pipe did not help.
@@ -235,8 +235,9 @@ __device__ __forceinline__ void walk(const T* p, int len, int tid, int step, One
 }
 
 // The teacher's side of a row over some of its entries, w = 2^((y - mx) k2):
-// S0 = sum w, S1 = sum w (y - mx) k2, S2 = sum w (x[id] - ref) k2, so that
-// sum p (log2 p - (x[id] - ref) k2) = (S1 - S2) / S0 - log2 S0.  S0 = 0: no entries.
+// S0 = sum w, S1 = sum w (y - mx) k2, S2 = sum w (x[id] - m) k2 with m the row's largest
+// logit (an offset of all logits, or a masked one among them, costs no precision), so
+// that sum p (log2 p - (x[id] - m) k2) = (S1 - S2) / S0 - log2 S0.  S0 = 0: no entries.
 struct Entries {
   float mx, s0, s1, s2;
 };
@@ -299,13 +300,22 @@ __global__ void __launch_bounds__(kThreads, (kFwdBlocks<T, W>))
         o.add_vecs<T, 1>(one, k2);
       });
   float2 ms = warp_join(make_float2(o.m, o.sum()), k2);
+  if constexpr (W > 1) {
+    if (lane == 0) part[warp] = ms;
+    __syncthreads();
+    ms = warp_join(lane < kWarps ? part[lane] : make_float2(-INFINITY, 0.f), k2);
+    if (split > 1) {
+      if (threadIdx.x == 0) mine = ms;
+      cluster_barrier();
+      if (rank == 0) ms = warp_join(lane < split ? ld_peer(&mine, (unsigned)lane) : make_float2(-INFINITY, 0.f), k2);
+      cluster_barrier();  // every block's `mine` has been read
+      if (rank != 0) return;
+    }
+  }
+  const float m = ms.x;
 
   Entries e{-INFINITY, 0.f, 0.f, 0.f};
-  // one of the row's logits: a common offset of all of them loses nothing
-  float ref = 0.f;
-  if (rank == 0 && (W == 1 || warp * 32 < t.K)) {
-    ref = to_f(x[0]);
-    if (!(fabsf(ref) <= kFar)) ref = 0.f;
+  if (W == 1 || warp * 32 < t.K) {
 #pragma unroll
     for (int i = 1; i < kPerThread; ++i) load_entry(i);
     float xg[kPerThread];
@@ -323,27 +333,15 @@ __global__ void __launch_bounds__(kThreads, (kFwdBlocks<T, W>))
       if (w == 0.f) continue;
       e.s0 += w;
       e.s1 += w * d;
-      e.s2 += w * ((xg[i] - ref) * k2);
+      e.s2 += w * ((xg[i] - m) * k2);
     }
     e.s0 = warp_sum(e.s0);
     e.s1 = warp_sum(e.s1);
     e.s2 = warp_sum(e.s2);
   }
   if constexpr (W > 1) {
-    if (lane == 0) {
-      part[warp] = ms;
-      entries[warp] = e;
-    }
+    if (lane == 0) entries[warp] = e;
     __syncthreads();
-    if (warp == 0) ms = warp_join(lane < kWarps ? part[lane] : make_float2(-INFINITY, 0.f), k2);
-    if (split > 1) {
-      if (threadIdx.x == 0) mine = ms;
-      cluster_barrier();
-      if (rank == 0 && warp == 0)
-        ms = warp_join(lane < split ? ld_peer(&mine, (unsigned)lane) : make_float2(-INFINITY, 0.f), k2);
-      cluster_barrier();  // every block's `mine` has been read
-      if (rank != 0) return;
-    }
     e = entries[0];  // every thread joins them, in one order
 #pragma unroll
     for (int w = 1; w < kWarps; ++w) e = join(e, entries[w], k2);
@@ -358,28 +356,18 @@ __global__ void __launch_bounds__(kThreads, (kFwdBlocks<T, W>))
     }
   }
   if (W > 1 && warp != 0) return;
-  const float m = ms.x;
-  float a = (e.s1 - e.s2) / e.s0 - log2f(e.s0);
-  float rest = fmaf(-ref, k2, base_of(m, k2));
+  float rest = fmaf(-m, k2, base_of(m, k2));  // the rounding of the base
   if (fabsf(m) > kFar && fabsf(m) < INFINITY) {  // differences to m first (this warp alone, the whole row)
     float s = 0.f;
     for (int i = lane; i < V; i += 32) s += fast_exp2((to_f(x[i]) - m) * k2);
     ms.y = warp_sum(s);
-    a = 0.f;
-    for (int k = lane; k < t.K; k += 32) {
-      const int v = teacher_id(t, row * t.K + k, V);
-      const float yk = teacher_logit(t, row * t.K + k);
-      if (v < 0 || yk == -INFINITY) continue;
-      const float lp = (yk - e.mx) * k2 - log2f(e.s0), pk = fast_exp2(lp);
-      if (pk != 0.f) a += pk * (lp - (to_f(x[v]) - m) * k2);
-    }
-    a = warp_sum(a);
     rest = 0.f;
   }
   if (lane == 0) {
     const float log2_s = log2f(ms.y);
     stats[row] = RowStats{base_of(m, k2), log2_s, m, some ? 1.f : 0.f};
-    // sum p (log2 p - log2 q) = sum p (log2 p - (x[id] - ref) k2) + (base - ref k2) + log2 s
+    // sum p (log2 p - log2 q) = sum p (log2 p - (x[id] - m) k2) + (base - m k2) + log2 s
+    const float a = (e.s1 - e.s2) / e.s0 - log2f(e.s0);
     loss[row] = some ? temp * temp * kLn2 * (a + (rest + log2_s)) : 0.f;
     counted[row] = some ? 1.f : 0.f;
   }

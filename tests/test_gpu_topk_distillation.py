@@ -264,3 +264,19 @@ def test_many_rows(dtype, N, V, K):
     ids[7] = ids[7, 0]
     ids[8, -1] = ids[8, 0]
     _compare(x, teacher, ids, 1.3, "none", torch.randn(N, device="cuda"))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("N,V,K", [(3, 60000, 40), (40, 1000, 7), (1800, 600, 7)])
+def test_masked_tokens_and_offsets_cost_no_precision(dtype, N, V, K):
+    """Large negative logits at the first tokens (a mask), a whole eighth of the
+    vocabulary or a listed token, and rows with a common offset."""
+    x, teacher, ids = _inputs(N, V, K, dtype, N, ragged=False)
+    mask = -6e4 if dtype == torch.float16 else -1e9
+    ids.clamp_(min=V // 8)  # listed tokens are not masked (a few are listed twice now)
+    x[:, 0] = mask
+    x[1, :V // 8] = mask
+    x[2] += 64.0
+    x[2, :3] = mask
+    _compare(x, teacher, ids, 1.7, "none", torch.randn(N, device="cuda"))
