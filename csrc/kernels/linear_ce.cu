@@ -106,35 +106,61 @@ __global__ void __launch_bounds__(1024) row_scale_kernel(const int64_t* __restri
   if (blockIdx.x == 0 && threadIdx.x == 0) alpha[0] = (g_per_row ? 1.f : g[0] * factor[0]) / f;
 }
 
-// out = alpha * (slice 0 + slice 1 + ...), rounded once.
-template <typename T>
+// out = alpha * (slice 0 + slice 1 + ...), rounded once.  G warps of a block share the
+// slices of 32 vectors, each a consecutive part of them, and are joined in order: with
+// many slices of a small product one thread a vector is one long chain of loads.
+template <typename T, int G>
 __global__ void __launch_bounds__(256) join_slices_kernel(const float4* __restrict__ c, int slices, int64_t n4,
                                                           const float* __restrict__ alpha, T* __restrict__ out) {
+  __shared__ float4 sh[8][32];
   const float a = alpha[0];
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n4; i += (int64_t)gridDim.x * 256) {
-    float4 v = c[i];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = warp % G;
+  constexpr int kVecs = 32 * 8 / G;  // vectors a block
+  for (int64_t i0 = (int64_t)blockIdx.x * kVecs; i0 < n4; i0 += (int64_t)gridDim.x * kVecs) {
+    const int64_t i = i0 + (warp / G) * 32 + lane;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (i < n4) {
 #pragma unroll 4
-    for (int s = 1; s < slices; ++s) {
-      const float4 w = c[s * n4 + i];
-      v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
+      for (int s = slices * part / G; s < slices * (part + 1) / G; ++s) {
+        const float4 w = c[s * n4 + i];
+        v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
+      }
     }
-    union { uint2 raw; T t[4]; } o;
-    o.t[0] = from_f<T>(v.x * a), o.t[1] = from_f<T>(v.y * a), o.t[2] = from_f<T>(v.z * a), o.t[3] = from_f<T>(v.w * a);
-    reinterpret_cast<uint2*>(out)[i] = o.raw;
+    if constexpr (G > 1) {
+      sh[warp][lane] = v;
+      __syncthreads();
+      if (part == 0) {
+#pragma unroll
+        for (int g = 1; g < G; ++g) {
+          const float4 w = sh[warp + g][lane];
+          v.x += w.x, v.y += w.y, v.z += w.z, v.w += w.w;
+        }
+      }
+      __syncthreads();
+    }
+    if (part == 0 && i < n4) {
+      union { uint2 raw; T t[4]; } o;
+      o.t[0] = from_f<T>(v.x * a), o.t[1] = from_f<T>(v.y * a), o.t[2] = from_f<T>(v.z * a), o.t[3] = from_f<T>(v.w * a);
+      reinterpret_cast<uint2*>(out)[i] = o.raw;
+    }
   }
 }
 
-void join_slices(const at::Tensor& c, int slices, const float* alpha, at::Tensor& out) {
+template <typename T>
+void join_slices_as(const at::Tensor& c, int slices, const float* alpha, at::Tensor& out) {
   const int64_t n4 = out.numel() / 4;
-  const unsigned blocks = (unsigned)std::min<int64_t>((n4 + 255) / 256, (int64_t)num_sms() * 16);
-  if (out.scalar_type() == at::kBFloat16)
-    join_slices_kernel<__nv_bfloat16><<<blocks, 256, 0, stream()>>>(
-        reinterpret_cast<const float4*>(c.data_ptr<float>()), slices, n4, alpha,
-        reinterpret_cast<__nv_bfloat16*>(out.data_ptr()));
-  else
-    join_slices_kernel<__half><<<blocks, 256, 0, stream()>>>(reinterpret_cast<const float4*>(c.data_ptr<float>()), slices,
-                                                             n4, alpha, reinterpret_cast<__half*>(out.data_ptr()));
+  const float4* p = reinterpret_cast<const float4*>(c.data_ptr<float>());
+  T* o = reinterpret_cast<T*>(out.data_ptr());
+  const auto blocks = [&](int64_t vecs) { return (unsigned)std::min<int64_t>((n4 + vecs - 1) / vecs, (int64_t)num_sms() * 16); };
+  // 512 x 256 outputs of 32 slices: 4.0 us by groups, 7.3 us by single threads
+  if (slices >= 8) join_slices_kernel<T, 8><<<blocks(32), 256, 0, stream()>>>(p, slices, n4, alpha, o);
+  else join_slices_kernel<T, 1><<<blocks(256), 256, 0, stream()>>>(p, slices, n4, alpha, o);
   LRB_LAUNCH_CHECK();
+}
+
+void join_slices(const at::Tensor& c, int slices, const float* alpha, at::Tensor& out) {
+  if (out.scalar_type() == at::kBFloat16) join_slices_as<__nv_bfloat16>(c, slices, alpha, out);
+  else join_slices_as<__half>(c, slices, alpha, out);
 }
 
 void check_head_inputs(const at::Tensor& h, const at::Tensor& w, const at::Tensor& targets) {
