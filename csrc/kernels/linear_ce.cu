@@ -14,10 +14,14 @@
 // products of the backward 1.60, 1.49 and 1.49 ms in 5 pieces, the step 6.8 ms under the
 // power cap (1.26 PFLOP/s; cuBLAS products alone sustain 1.37).
 //
+// The logits are the tensor cores' fp32 accumulators: against 64 bits the row losses are
+// off by 2-norm 4.6e-7 at d = 1024 and 1.8e-6 at d = 4096 (2.5e-7 and 5.7e-7 with fp32
+// multiply-adds), the accumulation cutting off what does not fit.
+//
 // dz is the one value that is rounded to 16 bits on the way: it is an operand of
 // the two gradient products, relative 2^-9 (bf16) or 2^-12 (fp16) an element.  For
-// fp16, whose smallest normal number is 6e-5, it is scaled by a power of two that
-// brings the largest |r_n| to [2^13, 2^14] and the products are scaled back.
+// fp16, whose smallest normal number is 6e-5, it is scaled so that the largest |r_n| is
+// 2^13 and the products are scaled back.
 #include "../common.cuh"
 
 #include <climits>
@@ -79,31 +83,28 @@ __global__ void __launch_bounds__(256) join_tiles_kernel(const float2* __restric
   counted[row] = c ? 1.f : 0.f;
 }
 
-// The weight of each row inside dz, and alpha, which the outputs are multiplied by.
-// One weight for all rows (a sum or a mean) goes into alpha: dz = softmax - onehot then
-// rounds an improbable target to exactly -1, where -1 times the weight would round the
-// same way in every row (2-norm error of the gradients of a 512 x 32000 bf16 mean
-// 2.3e-3 instead of 1.9e-3).  `normalise` (fp16): the power of two f described above.
+// The weight of each row inside dz, and alpha, which the outputs are multiplied by.  The
+// largest weight (the only one of a sum or a mean) goes into alpha: dz = softmax - onehot
+// then rounds an improbable target to exactly -1, where -1 times a weight that all rows
+// share would round the same way in every row (2-norm error of the gradients of a
+// 512 x 32000 bf16 mean 2.3e-3 instead of 1.9e-3).  f: the power of two of fp16.
 __global__ void __launch_bounds__(1024) row_scale_kernel(const int64_t* __restrict__ targets, int64_t n, int64_t V,
                                                          int64_t ignore, const float* __restrict__ g, int g_per_row,
-                                                         const float* __restrict__ factor, int normalise,
+                                                         const float* __restrict__ factor, float f,
                                                          float* __restrict__ row_scale, float* __restrict__ alpha) {
   __shared__ float red[32];
-  float f = normalise ? 8192.f : 1.f;
-  if (normalise && g_per_row) {  // every block finds it for itself
-    float mx = 0.f;
+  float most = g_per_row ? 0.f : g[0] * factor[0];
+  float inv = f;
+  if (g_per_row) {  // every block finds it for itself
     for (int64_t i = threadIdx.x; i < n; i += 1024)
-      if (counts(targets[i], ignore, V)) mx = fmaxf(mx, fabsf(g[i]));
-    mx = block_max(mx, red);
-    if (mx > 0.f && mx < INFINITY) {
-      int e;
-      frexpf(mx, &e);
-      f = ldexpf(1.f, min(max(14 - e, -100), 100));
-    }
+      if (counts(targets[i], ignore, V)) most = fmaxf(most, fabsf(g[i]));
+    most = block_max(most, red);
+    if (!(most > 1e-30f && most < INFINITY)) most = 1.f;  // nothing, or no number to divide by
+    inv = f / most;
   }
   for (int64_t i = (int64_t)blockIdx.x * 1024 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 1024)
-    row_scale[i] = counts(targets[i], ignore, V) ? (g_per_row ? g[i] * f : f) : 0.f;
-  if (blockIdx.x == 0 && threadIdx.x == 0) alpha[0] = (g_per_row ? 1.f : g[0] * factor[0]) / f;
+    row_scale[i] = counts(targets[i], ignore, V) ? (g_per_row ? g[i] * inv : f) : 0.f;
+  if (blockIdx.x == 0 && threadIdx.x == 0) alpha[0] = most / f;
 }
 
 // out = alpha * (slice 0 + slice 1 + ...), rounded once.  G warps of a block share the
@@ -227,10 +228,9 @@ std::tuple<at::Tensor, at::Tensor> linear_ce_bwd(const at::Tensor& h, const at::
   auto f32 = h.options().dtype(at::kFloat);
   auto scale = at::empty({n + 1}, f32);  // row scales, then alpha
   const float* alpha = scale.data_ptr<float>() + n;
-  const bool normalise = h.scalar_type() == at::kHalf;
   row_scale_kernel<<<(unsigned)std::min<int64_t>((n + 1023) / 1024, num_sms()), 1024, 0, stream()>>>(
       targets.data_ptr<int64_t>(), n, V, ignore, g.data_ptr<float>(), g_per_row ? 1 : 0,
-      g_per_row ? nullptr : factor.data_ptr<float>(), normalise ? 1 : 0, scale.data_ptr<float>(),
+      g_per_row ? nullptr : factor.data_ptr<float>(), h.scalar_type() == at::kHalf ? 8192.f : 1.f, scale.data_ptr<float>(),
       scale.data_ptr<float>() + n);
   LRB_LAUNCH_CHECK();
   if (piece == 0) piece = gemm_pair_ce_piece(n, V, d, 256 << 20, dev);

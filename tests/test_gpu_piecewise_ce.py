@@ -188,6 +188,21 @@ def test_small_and_large_row_weights(dtype, scale):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("weight", [0.7, -3e-5, 1e-35])
+def test_one_weight_for_all_rows(dtype, weight):
+    """Row losses with one upstream weight (``rows.mean()``) have the gradients of the sum
+    with it, to the bit: the weight is not rounded into the 16-bit logits' gradient."""
+    h, w, t = _inputs(200, 900, 64, dtype, 21)
+    g = torch.full((200,), abs(weight), device="cuda")
+    _, dh, dw = _run(h, w, t, "none", g)
+    _, dh2, dw2 = _run(h, w, t, "sum", g[0])
+    if weight > 1e-30 or weight < 0:
+        assert torch.equal(dh, dh2) and torch.equal(dw, dw2)
+    _compare(h, w, t, "none", weight * g / g[0])
+
+
+@pytest.mark.gpu
 def test_extreme_logits():
     """Peaked rows, and infinities in rows that count: the loss of the other rows stays."""
     from llm_research_b200 import ops
