@@ -12,9 +12,12 @@
 // a running sum per thread and joins them; the backward needs four numbers a row and
 // the probabilities p.  Everything is fp32, in powers of two with k2 = log2(e) / T:
 // with B = m k2 rounded once (any reference near the maximum would do, as long as both
-// sides use the same), log2 q_j = (x_j k2 - B) - log2 s, the bracket one fma.
-// Rows whose maximum is beyond 1e30, where x k2 - B would overflow (a row of the
-// type's lowest values), take differences x - m first.
+// sides use the same), log2 q_j = (x_j k2 - B) - log2 s, the bracket one fma.  At the
+// maximum the bracket is the rounding error of B, up to half a step of it, which grows
+// with |m|: within F = 2^22 / k2 it stays below 1/4.  So B is taken from m kept within
+// +-F (far_limit); what lies below -F (a mask) adds 2^-huge = 0 beside any logit above.
+// Rows whose maximum is itself beyond F (rows that hold nothing but a mask, or a huge
+// offset) take differences x - m first, in a second walk of the forward.
 //
 // Bounded by the bytes of the logits: 16384 x 32000 bf16 with 64 entries forward 196 to
 // 204 us (5.1 to 5.4 TB/s) and backward 317 us (6.6 TB/s), 4093 x 100287 fp32 with 200 entries 261 us
@@ -33,17 +36,16 @@ constexpr int kPerThread = 4;                   // teacher entries a thread hold
 constexpr int kMaxK = kPerThread * kThreads;    // entries of a row, for a block a row
 constexpr int kWarpK = kPerThread * 32;         // for a warp a row
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-constexpr float kFar = 1e30f;
 
 // Vectors in flight a thread (U) and blocks an SM, measured.  Forward: 16384 x 32000 bf16
 // 196 us at 4 / 6 (212 at 4 / 5, 194 at 4 / 8; a warp a row 199 at 8 / 4), 2048 x 100287
 // bf16 80 us at 4 / 6 (79 at 4 / 5, 83 at 4 / 8); 4093 x 100287 fp32 261 us at 8 / 4 (291 at
-// 4 / 6).  Backward: 320 us at 4 / 5 (335 at 4 / 8, 338 at 8 / 4), fp32 559 us at 4 / any
+// 4 / 6).  Backward: 320 us at 4 / 5 (335 at 4 / 8, 338 at 8 / 4), fp32 559 us at 4 / 4
 // (587 at 4 / 5).
 template <typename T, int W> constexpr int kFwdU = W == 1 || sizeof(T) == 4 ? 8 : 4;
 template <typename T, int W> constexpr int kFwdBlocks = W == 1 || sizeof(T) == 4 ? 4 : 6;
 template <typename T, int W> constexpr int kBwdU = W == 1 ? 8 : 4;
-template <typename T, int W> constexpr int kBwdBlocks = W == 1 ? 4 : sizeof(T) == 4 ? 1 : 5;
+template <typename T, int W> constexpr int kBwdBlocks = W == 1 || sizeof(T) == 4 ? 4 : 5;
 
 struct Teacher {
   const void* logits;  // (N, K) bf16 / fp16 / fp32
@@ -126,12 +128,19 @@ template <> struct Pairs<float> {
   }
 };
 
+// The largest maximum with a base of its own: |base| <= 2^22, finite for every k2.
+__device__ __forceinline__ float far_limit(float k2) { return fminf(__fdividef(4194304.f, k2), 1e30f); }
+
 // The base that goes with a maximum.  Rounded here: contracted into a following
-// subtraction, the bases of one maximum would differ by their rounding (1e22 at 1e30).
-__device__ __forceinline__ float base_of(float m, float k2) { return __fmul_rn(fminf(fmaxf(m, -kFar), kFar), k2); }
+// subtraction, the bases of one maximum would differ by their rounding.
+__device__ __forceinline__ float base_of(float m, float k2) {
+  const float f = far_limit(k2);
+  return __fmul_rn(fminf(fmaxf(m, -f), f), k2);
+}
 
 // Running maximum m and sum of 2^(x k2 - base), base = ref k2 with ref the maximum kept
-// within +-1e30: below, everything so far adds nothing (2^-huge = 0), and a NaN shows.
+// within +-far_limit: below, everything so far adds nothing beside a larger logit
+// (2^-huge = 0), and a NaN shows.
 struct Online {
   float m = -INFINITY, base;
   uint64_t s = 0;  // two partial sums
@@ -357,7 +366,7 @@ __global__ void __launch_bounds__(kThreads, (kFwdBlocks<T, W>))
   }
   if (W > 1 && warp != 0) return;
   float rest = fmaf(-m, k2, base_of(m, k2));  // the rounding of the base
-  if (fabsf(m) > kFar && fabsf(m) < INFINITY) {  // differences to m first (this warp alone, the whole row)
+  if (fabsf(m) > far_limit(k2) && fabsf(m) < INFINITY) {  // differences to m first (this warp alone, the whole row)
     float s = 0.f;
     for (int i = lane; i < V; i += 32) s += fast_exp2((to_f(x[i]) - m) * k2);
     ms.y = warp_sum(s);
@@ -443,7 +452,7 @@ __global__ void __launch_bounds__(kThreads, (kBwdBlocks<T, W>))
   }
   const float k2 = kLog2e / temp;
   const float coef = temp * (g_per_row ? g[row] : g[0] * factor[0]);
-  const bool far = !(fabsf(m) <= kFar);
+  const bool far = !(fabsf(m) <= far_limit(k2));
   const auto q = [&](float v) { return fast_exp2((far ? (v - m) * k2 : fmaf(v, k2, -base)) - l2); };
 
   // The entries of this range: the first of each thread (mostly the only one) is loaded

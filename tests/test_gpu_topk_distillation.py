@@ -280,3 +280,70 @@ def test_masked_tokens_and_offsets_cost_no_precision(dtype, N, V, K):
     x[2] += 64.0
     x[2, :3] = mask
     _compare(x, teacher, ids, 1.7, "none", torch.randn(N, device="cuda"))
+
+
+def _compare_rows(loss, dx, x, teacher, ids, T, g):
+    """Row losses and their gradient against ``_exact``.  Its bound leaves out that the
+    exponent (t - t_max) log2(e) / T of a probability p = e^(...) / S is rounded four times in
+    fp32 (log2 e, its division by T, the difference, the product), each by up to 2^-24 of it:
+    relative to p that is (t_max - t) / T 2^-22, 2^-18.5 for T = 0.5 and logits 6 apart.  And
+    it leaves out that an exponential, or a product with it, below the smallest normal
+    number 2^-126 is 0."""
+    (l, el), (d, ed) = _exact(x, teacher, ids, T, "none", g)
+    y = teacher.double() / T
+    span = y.amax(1, keepdim=True) - y
+    ep = T * g.double().abs()[:, None] * torch.softmax(y, 1) * span * 2.0 ** -22
+    ed = ed + torch.zeros_like(ed).scatter_add_(1, ids, ep) + (T * g.double().abs()[:, None] + 1) * 2.0 ** -126
+    _check("loss", loss, l, el)
+    _check("dx", dx, d, ed)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("N,V,K", [(12, 60000, 40), (40, 1001, 7), (1800, 600, 7)])
+@pytest.mark.parametrize("mask", [-1e10, -1e12, -1e20, -1e30, None])
+@pytest.mark.parametrize("T", [0.5, 1.0, 2.0, 3.5])
+def test_masks_of_any_size(dtype, N, V, K, mask, T):
+    """Masks from -1e10 to the type's lowest value (None) at the first, the last and a
+    listed token, over a stretch, and rows that hold nothing else.
+
+    The loss and the gradient do not change with a row's offset.  The rows of large
+    values are compared with the same rows less their largest value: the differences are
+    exact (equal values, values within a factor of two, or a mask that takes the other
+    one in whole), and the bounds are those of the small values."""
+    x, teacher, ids = _inputs(N, V, K, dtype, N, ragged=False)
+    low = torch.finfo(dtype).min if mask is None else mask
+    ids.clamp_(min=V // 8, max=V - 2)  # the listed tokens are not masked
+    x[0, 0] = low
+    x[1, -1] = low
+    x[2, ids[2, 0]] = max(low, -1e30)  # times T, the lowest value would leave fp32
+    x[3, :V // 8] = low
+    x[4, 0], x[4, -1], x[4, 1:9] = low, low, float("-inf")
+    x[5] = low                         # uniform
+    x[6] = low
+    x[6, V // 2:] = low * (1 - 2.0 ** -6)  # uniform over a half, the rest adds nothing
+    ids[6] = V // 2 + torch.arange(K, device="cuda")
+    x[7] = abs(low)
+    g = torch.randn(N, device="cuda")
+    loss, dx = _run(x, teacher, ids, T, "none", g)
+    near = x.clone()
+    near[5:8] -= x[5:8].amax(1, keepdim=True)
+    _compare_rows(loss, dx, near, teacher, ids, T, g)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("N,V", [(26, 40000), (26, 777), (1800, 300)])
+@pytest.mark.parametrize("T", [0.01, 1.0, 3.5])
+def test_large_offsets(N, V, T):
+    """Rows around an offset of 2^14 to 2^26, either sign: each small difference is exact
+    in fp32 there, and costs no precision."""
+    x, teacher, ids = _inputs(N, V, 9, torch.float32, 5, ragged=False)
+    step = torch.randint(0, 8, (N, V), device="cuda", generator=torch.Generator("cuda").manual_seed(2)).float()
+    for r in range(26):
+        offset = 2.0 ** (14 + r // 2)
+        unit = max(1.0, offset * 2.0 ** -22)
+        x[r] = (offset if r % 2 else -offset) + unit * step[r]
+    g = torch.randn(N, device="cuda")
+    loss, dx = _run(x, teacher, ids, T, "none", g)
+    near = x - x.amax(1, keepdim=True)
+    _compare_rows(loss, dx, near, teacher, ids, T, g)
