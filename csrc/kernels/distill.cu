@@ -602,7 +602,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> distill_f
   const Rows rows = make_rows(logits, "topk_distillation");
   const int64_t n = logits.size(0) * logits.size(1), V = logits.size(2);
   const Teacher t = make_teacher(t_logits, t_ids, logits, n, "topk_distillation");
-  LRB_CHECK(temperature > 0.0 && std::isfinite(temperature), "topk_distillation: temperature must be positive");
+  LRB_CHECK(temperature >= 1e-18 && temperature <= 1e18,  // T, T^2 and log2(e) / T are normal fp32 numbers
+            "topk_distillation: temperature must be between 1e-18 and 1e18");
   c10::cuda::CUDAGuard g(logits.device());
   bind_device(logits.get_device());
   auto f32 = logits.options().dtype(at::kFloat);

@@ -13,7 +13,9 @@ listed twice has the sum of its probabilities.  The teacher gets no gradient.
 
 CUDA (``csrc/kernels/distill.cu``): the forward reads the logits once and keeps
 four numbers a row and the teacher's probabilities; the backward reads them once and writes the gradient; fp32
-arithmetic for bf16, fp16 and fp32 logits.  The full-vocabulary form of the
+arithmetic for bf16, fp16 and fp32 logits: a row's loss is off by some ``T^2 2^-20``
+times the sizes of its logarithms, which is much beside the loss itself once ``T``
+flattens both distributions (hundreds).  The full-vocabulary form of the
 same loss is ``VerificationDistillation.temperature_scaled_loss``.
 """
 
@@ -28,6 +30,7 @@ from llm_research_b200._ext import native
 _REDUCTIONS = {"none": 0, "sum": 1, "mean": 2}
 _DTYPES = (torch.bfloat16, torch.float16, torch.float32)
 MAX_TEACHER_ENTRIES = 1024
+MIN_TEMPERATURE, MAX_TEMPERATURE = 1e-18, 1e18
 
 
 def _plain(x, teacher, ids, T, reduction):
@@ -51,12 +54,20 @@ def _plain(x, teacher, ids, T, reduction):
     return rows.sum() if reduction == "sum" else rows.sum() / some.sum().clamp(min=1)
 
 
+def check_cuda_temperature(T: float) -> None:
+    """The kernels hold ``T``, ``T^2`` and ``log2(e) / T`` in fp32: each has to be a normal number."""
+    if not MIN_TEMPERATURE <= T <= MAX_TEMPERATURE:
+        raise ValueError(f"topk_distillation: temperature must be between {MIN_TEMPERATURE:g} and "
+                         f"{MAX_TEMPERATURE:g} on CUDA, got {T:g}")
+
+
 def topk_distillation(logits: torch.Tensor, teacher_logits: torch.Tensor, teacher_ids: torch.Tensor,
                       temperature: float = 1.0, reduction: str = "mean") -> torch.Tensor:
     """``logits`` ``(..., V)``; ``teacher_logits``, ``teacher_ids`` ``(..., K)`` with
     the same leading shape (ids int64 or int32).  ``reduction``: ``"mean"`` over the
     rows that have entries (0 without any), ``"sum"``, or ``"none"`` (the leading
-    shape), fp32.  See the module docstring."""
+    shape), fp32.  ``temperature`` from 1e-18 to 1e18 and at most 1024 entries a row on
+    CUDA.  See the module docstring."""
     T = float(temperature)
     if not (T > 0.0 and math.isfinite(T)):
         raise ValueError(f"topk_distillation: temperature must be positive and finite, got {temperature}")
@@ -72,6 +83,7 @@ def topk_distillation(logits: torch.Tensor, teacher_logits: torch.Tensor, teache
     if not logits.is_cuda:
         rows = _plain(logits.reshape(-1, V), teacher_logits.reshape(-1, K), teacher_ids.reshape(-1, K), T, reduction)
         return rows.reshape(lead) if reduction == "none" else rows
+    check_cuda_temperature(T)
     if K > MAX_TEACHER_ENTRIES:
         raise ValueError(f"topk_distillation: at most {MAX_TEACHER_ENTRIES} teacher entries on CUDA, got {K}")
     for name, t in (("logits", logits), ("teacher_logits", teacher_logits)):

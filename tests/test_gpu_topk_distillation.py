@@ -347,3 +347,24 @@ def test_large_offsets(N, V, T):
     loss, dx = _run(x, teacher, ids, T, "none", g)
     near = x - x.amax(1, keepdim=True)
     _compare_rows(loss, dx, near, teacher, ids, T, g)
+
+
+def test_temperature_that_leaves_fp32_is_refused():
+    """On CUDA the temperature and its square are fp32 numbers."""
+    from llm_research_b200.ops.distill import check_cuda_temperature
+
+    for T in (1e-18, 1e-3, 1.0, 1e18):
+        check_cuda_temperature(T)
+    for T in (1e-46, 1e-20, 1e20, 1e39):
+        with pytest.raises(ValueError, match="temperature"):
+            check_cuda_temperature(T)
+
+
+@pytest.mark.gpu
+def test_temperature_that_leaves_fp32_is_refused_on_cuda():
+    from llm_research_b200 import ops
+
+    x, teacher, ids = _inputs(3, 50, 2, torch.float32, 0)
+    for T in (1e-46, 1e-20, 1e20, 1e39):
+        with pytest.raises(ValueError, match="temperature"):
+            ops.topk_distillation(x, teacher, ids, T)
