@@ -5,6 +5,7 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
+#include <initializer_list>
 #include <memory>
 #include <tuple>
 
@@ -43,7 +44,20 @@ variable_list once(const char* name, variable_list grads) {
 
 at::Tensor unit_columns(const at::Tensor& t) { return t.stride(-1) == 1 || t.size(-1) <= 1 ? t : t.contiguous(); }
 
-struct EmbeddingGradFn;
+// Forward mode: the kernels see values only, so a tangent is followed (the lookup, which
+// is linear) or refused.  Detached values have none.
+bool has_tangent(const at::Tensor& t) { return t._fw_grad(0).defined(); }
+
+void refuse_tangents(const char* name, std::initializer_list<at::Tensor> inputs) {
+  for (const auto& t : inputs)
+    TORCH_CHECK_NOT_IMPLEMENTED(!has_tangent(t), name, " has no forward-mode derivative");
+}
+
+bool tracked(const at::Tensor& t) { return at::GradMode::is_enabled() && t.requires_grad(); }
+
+// scale * w[ids], and the gradient of w, with their derivatives of both modes.
+at::Tensor lookup(const at::Tensor& w, const at::Tensor& ids, double scale, int64_t padding);
+at::Tensor table_gradient(const at::Tensor& dy, const at::Tensor& ids, int64_t rows, double scale, int64_t padding);
 
 struct EmbeddingFn : public Function<EmbeddingFn> {
   static Variable forward(AutogradContext* ctx, const Variable& w, const Variable& ids, double scale, int64_t padding) {
@@ -70,7 +84,7 @@ struct EmbeddingGradFn : public Function<EmbeddingGradFn> {
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     const auto ids = ctx->get_saved_variables()[0];
     const int64_t padding = ctx->saved_data["padding"].toInt();
-    const auto out = EmbeddingFn::apply(g[0].contiguous(), ids, ctx->saved_data["scale"].toDouble(), padding);
+    const auto out = lookup(g[0], ids, ctx->saved_data["scale"].toDouble(), padding);
     const auto kept = ids.ge(0).logical_and(ids.lt(ctx->saved_data["rows"].toInt())).logical_and(ids.ne(padding));
     return {at::where(kept.unsqueeze(1), out, at::zeros({}, out.options())), Variable(), Variable(), Variable(),
             Variable()};
@@ -79,11 +93,28 @@ struct EmbeddingGradFn : public Function<EmbeddingGradFn> {
 
 variable_list EmbeddingFn::backward(AutogradContext* ctx, variable_list g) {
   const auto ids = ctx->get_saved_variables()[0];
-  const int64_t rows = ctx->saved_data["rows"].toInt(), padding = ctx->saved_data["padding"].toInt();
-  const double scale = ctx->saved_data["scale"].toDouble();
-  const auto dw = at::GradMode::is_enabled() ? EmbeddingGradFn::apply(g[0], ids, rows, scale, padding)
-                                             : embedding_bwd(unit_columns(g[0]), ids, rows, padding, scale);
-  return {dw, Variable(), Variable(), Variable()};
+  return {table_gradient(g[0], ids, ctx->saved_data["rows"].toInt(), ctx->saved_data["scale"].toDouble(),
+                         ctx->saved_data["padding"].toInt()),
+          Variable(), Variable(), Variable()};
+}
+
+at::Tensor lookup(const at::Tensor& w, const at::Tensor& ids, double scale, int64_t padding) {
+  if (has_tangent(w)) {
+    const auto [value, tangent] = at::_unpack_dual(w, 0);
+    return at::_make_dual(lookup(value, ids, scale, padding), lookup(tangent, ids, scale, padding), 0);
+  }
+  const at::Tensor table = unit_columns(w);
+  return tracked(table) ? EmbeddingFn::apply(table, ids, scale, padding) : embedding_fwd(ids, table, scale);
+}
+
+at::Tensor table_gradient(const at::Tensor& dy, const at::Tensor& ids, int64_t rows, double scale, int64_t padding) {
+  if (has_tangent(dy)) {
+    const auto [value, tangent] = at::_unpack_dual(dy, 0);
+    return at::_make_dual(table_gradient(value, ids, rows, scale, padding),
+                          table_gradient(tangent, ids, rows, scale, padding), 0);
+  }
+  return at::GradMode::is_enabled() ? EmbeddingGradFn::apply(dy, ids, rows, scale, padding)
+                                    : embedding_bwd(unit_columns(dy), ids, rows, padding, scale);
 }
 
 struct LinearCEFn : public Function<LinearCEFn> {
@@ -97,6 +128,7 @@ struct LinearCEFn : public Function<LinearCEFn> {
     return reduction == 0 ? rows : out;
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
+    refuse_tangents("piecewise_linear_cross_entropy", {g[0]});
     const auto s = ctx->get_saved_variables();
     const bool per_row = ctx->saved_data["per_row"].toBool(), need_h = ctx->needs_input_grad(0),
                need_w = ctx->needs_input_grad(1);
@@ -123,6 +155,7 @@ struct DistillFn : public Function<DistillFn> {
     return reduction == 0 ? rows : out;
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
+    refuse_tangents("topk_distillation", {g[0]});
     const auto s = ctx->get_saved_variables();
     const bool per_row = ctx->saved_data["per_row"].toBool();
     at::Tensor dx;
@@ -135,16 +168,12 @@ struct DistillFn : public Function<DistillFn> {
   }
 };
 
-bool tracked(const at::Tensor& t) { return at::GradMode::is_enabled() && t.requires_grad(); }
-
 }  // namespace
 
 // `ids` of any shape and strides; out (*ids.shape, d).
 at::Tensor embedding(const at::Tensor& ids, const at::Tensor& w, double scale, int64_t padding) {
   const at::Tensor flat = (ids.dim() == 1 ? ids : ids.reshape({-1})).contiguous();
-  const at::Tensor table = unit_columns(w);
-  const at::Tensor out =
-      tracked(table) ? EmbeddingFn::apply(table, flat, scale, padding) : embedding_fwd(flat, table, scale);
+  const at::Tensor out = lookup(w, flat, scale, padding);
   if (ids.dim() == 1) return out;
   auto shape = ids.sizes().vec();
   shape.push_back(w.size(1));
@@ -154,6 +183,7 @@ at::Tensor embedding(const at::Tensor& ids, const at::Tensor& w, double scale, i
 // h (..., d), targets of its leading shape; a row loss for each target with reduction 0.
 at::Tensor piecewise_linear_ce(const at::Tensor& h, const at::Tensor& w, const at::Tensor& targets, int64_t ignore,
                                int64_t reduction, int64_t piece) {
+  refuse_tangents("piecewise_linear_cross_entropy", {h, w});
   const auto rows16 = [](const at::Tensor& t) {  // rows that the tensor maps take: 16-byte aligned, unit columns
     return t.stride(1) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 &&
                    t.stride(0) * (int64_t)t.element_size() % 16 == 0 && (t.stride(0) >= t.size(1) || t.size(0) <= 1)
@@ -176,6 +206,7 @@ at::Tensor piecewise_linear_ce(const at::Tensor& h, const at::Tensor& w, const a
 // dimensions are read in place.
 at::Tensor topk_distillation(const at::Tensor& x, const at::Tensor& teacher, const at::Tensor& ids, double temperature,
                              int64_t reduction) {
+  refuse_tangents("topk_distillation", {x});
   const int64_t V = x.size(-1), K = ids.size(-1);
   const at::Tensor x3 = unit_columns(x.dim() == 3 ? x : x.dim() == 2 ? x.unsqueeze(0) : x.reshape({1, -1, V}));
   const at::Tensor t2 = (teacher.dim() == 2 ? teacher : teacher.reshape({-1, K})).detach().contiguous(),

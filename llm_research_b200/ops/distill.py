@@ -10,6 +10,7 @@ An entry counts when ``0 <= id_k < V`` and ``t_k`` is not ``-inf``: shorter list
 are padded with the id -1 (what stands in a padded place is not looked at).  A
 row without entries has loss 0, gradient 0 and is left out of the mean.  A token
 listed twice has the sum of its probabilities.  The teacher gets no gradient.
+On CUDA the loss can be differentiated once, in reverse mode (anything else raises).
 
 CUDA (``csrc/kernels/distill.cu``): the forward reads the logits once and keeps
 four numbers a row and the teacher's probabilities; the backward reads them once and writes the gradient; fp32

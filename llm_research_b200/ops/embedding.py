@@ -6,8 +6,9 @@ sums in fp32, one rounding to the weight's dtype (bf16, fp16 or fp32).
 
 CUDA (``csrc/kernels/embedding.cu``): the lookup is one kernel; the gradient
 sorts the tokens (one cluster, stable) and adds the occurrences of a token in the
-order of their positions: the same inputs give the same bits.  ``padding_idx`` only leaves its row out of the gradient
-(``F.embedding`` semantics).  An id outside ``[0, V)`` cannot be reported from
+order of their positions: the same inputs give the same bits.  The lookup and its
+gradient carry forward-mode tangents, and can be differentiated again.
+``padding_idx`` only leaves its row out of the gradient (``F.embedding`` semantics).  An id outside ``[0, V)`` cannot be reported from
 the device without a synchronisation: its output row is NaN and it has no
 gradient (on the CPU it raises ``IndexError``).
 """

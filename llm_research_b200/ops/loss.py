@@ -156,7 +156,8 @@ def piecewise_linear_cross_entropy(h: torch.Tensor, w: torch.Tensor, targets: to
     the log-sum-exp is taken from the fp32 products, and the backward forms the
     logits' gradient for ``piece`` vocabulary rows at a time (default: a buffer of
     at most 256 MB, or 1024 rows).  As in any matrix product, an ``inf`` or NaN in a row of ``h``
-    that does not count still reaches ``dw`` (0 * inf)."""
+    that does not count still reaches ``dw`` (0 * inf).  On CUDA the loss can be
+    differentiated once, in reverse mode (anything else raises)."""
     if reduction not in _REDUCTIONS:
         raise ValueError(f"piecewise_linear_cross_entropy: reduction must be one of {sorted(_REDUCTIONS)}, "
                          f"got {reduction!r}")

@@ -256,3 +256,30 @@ def test_shared_embeddings_use_the_kernel_and_keep_their_results():
         out.backward(dy)
         _check_grad(m.weight.grad, dy, ids, 400, 1.0, padding=3)
         assert (m.weight.grad[3] == 0).all()
+
+
+@pytest.mark.gpu
+def test_forward_mode_derivative_is_the_lookup_of_the_tangent():
+    import torch.autograd.forward_ad as fw
+
+    from llm_research_b200 import ops
+
+    g = torch.Generator("cuda").manual_seed(9)
+    w, t = (torch.randn(20, 24, device="cuda", generator=g) for _ in range(2))
+    ids = torch.tensor([[3, 0, 3], [19, 7, 5]], device="cuda")
+    dy, dyt = (torch.randn(2, 3, 24, device="cuda", generator=g) for _ in range(2))
+    for grad in (False, True):
+        with fw.dual_level():
+            w1 = w.clone().requires_grad_(grad)
+            out = fw.unpack_dual(ops.embedding(ids, fw.make_dual(w1, t), 1.5, padding_idx=3))
+            assert torch.equal(out.primal, 1.5 * w[ids]) and torch.equal(out.tangent, 1.5 * t[ids])
+            if grad:
+                dw, = torch.autograd.grad(out.primal, w1, dy)
+                _check_grad(dw, dy, ids, 20, 1.5, padding=3)
+    w.requires_grad_()
+    for create_graph in (False, True):  # the gradient is linear in dy as well
+        with fw.dual_level():
+            out = ops.embedding(ids, w, 1.5, padding_idx=3)
+            dw = fw.unpack_dual(torch.autograd.grad(out, w, fw.make_dual(dy, dyt), create_graph=create_graph)[0])
+            _check_grad(dw.primal, dy, ids, 20, 1.5, padding=3)
+            _check_grad(dw.tangent, dyt, ids, 20, 1.5, padding=3)

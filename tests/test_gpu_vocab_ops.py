@@ -316,3 +316,29 @@ def test_offsets_past_32_bits():
     ref, = torch.autograd.grad(want, tail)
     assert (dx[-2:].double() - ref).abs().max() <= 2 ** -9 * ref.abs().max() + 1e-6
     assert rows[:-2].eq(0).all() and not dx[:-2].any()
+
+
+@pytest.mark.gpu
+def test_losses_refuse_forward_mode():
+    import torch.autograd.forward_ad as fw
+
+    from llm_research_b200 import ops
+
+    ids, w, mix, targets, teacher, tids = _inputs("cuda", torch.bfloat16)
+    h = (0.1 * torch.randn(96, 64, device="cuda")).bfloat16()
+    x = h @ w.t()
+    one = torch.ones((), device="cuda")
+    for grad in (False, True):
+        for f, leaf in ((lambda a: ops.piecewise_linear_cross_entropy(a, w, targets), h),
+                        (lambda a: ops.piecewise_linear_cross_entropy(h, a, targets), w),
+                        (lambda a: ops.topk_distillation(a, teacher, tids), x)):
+            with fw.dual_level():
+                a = leaf.clone().requires_grad_(grad)
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    f(fw.make_dual(a, torch.ones_like(a)))
+                if grad:
+                    with pytest.raises(RuntimeError, match="forward-mode"):
+                        torch.autograd.grad(f(a), a, fw.make_dual(one, one))
+    with fw.dual_level():  # the teacher is a constant in both modes
+        loss = ops.topk_distillation(x, fw.make_dual(teacher, torch.ones_like(teacher)), tids)
+        assert fw.unpack_dual(loss).tangent is None and torch.equal(loss, ops.topk_distillation(x, teacher, tids))
