@@ -283,3 +283,98 @@ def test_forward_mode_derivative_is_the_lookup_of_the_tangent():
             dw = fw.unpack_dual(torch.autograd.grad(out, w, fw.make_dual(dy, dyt), create_graph=create_graph)[0])
             _check_grad(dw.primal, dy, ids, 20, 1.5, padding=3)
             _check_grad(dw.tangent, dyt, ids, 20, 1.5, padding=3)
+
+
+# ------------------------------------------------------------------ SharedEmbeddings as a module
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+
+
+def _shared(device, **kw):
+    from genesis.model.embeddings import SharedEmbeddings
+
+    torch.manual_seed(2)
+    m = SharedEmbeddings(40, 16, **kw).to(device)
+    return m, torch.tensor([[1, 5, 5], [39, 0, 2]], device=device)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+@pytest.mark.parametrize("scale", [1.0, 4.0])
+def test_hooks_and_replacements_of_the_inner_embedding_act(device, scale):
+    """Hooks see the rows of the table; the scale comes behind them."""
+    m, ids = _shared(device, scale=scale)
+    want, rows, seen = m(ids), m.weight[ids], []
+    pre = m.embedding.register_forward_pre_hook(lambda mod, args: seen.append("pre") or (args[0] * 0 + 5,))
+    post = m.embedding.register_forward_hook(lambda mod, args, out: out + 1)
+    assert torch.equal(m(ids), ((m.weight[5] + 1) * scale).expand(2, 3, 16)) and seen == ["pre"]
+    pre.remove(), post.remove()
+    back = m.embedding.register_full_backward_hook(lambda mod, gin, gout: seen.append(gout[0].clone()))
+    m(ids).sum().backward()
+    assert seen[1].eq(scale).all()
+    back.remove()
+    every = torch.nn.modules.module.register_module_forward_hook(
+        lambda mod, args, out: seen.append(out) if mod is m.embedding else None)
+    assert torch.equal(m(ids), want) and torch.equal(seen[2], rows)
+    every.remove()
+    assert torch.equal(m(ids), want) and len(seen) == 3
+    other = torch.nn.Embedding(40, 16).to(device)
+    inner, m.embedding = m.embedding, other
+    assert torch.equal(m(ids), other(ids) * scale)
+
+    class Shifted(torch.nn.Embedding):
+        def forward(self, i):
+            return super().forward(i) + 1
+
+    m.embedding = Shifted(40, 16).to(device)
+    assert torch.equal(m(ids), (m.weight[ids] + 1) * scale)
+    m.embedding = inner
+    inner.forward = lambda i: torch.ones(*i.shape, 16, device=device)
+    assert m(ids).eq(scale).all() and m(ids).shape == (2, 3, 16)
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_settings_of_the_inner_embedding_act(device):
+    F = torch.nn.functional
+    m, ids = _shared(device)
+    dy = torch.randn(2, 3, 16, device=device)
+    m.embedding.scale_grad_by_freq = True
+    w = m.weight.detach().clone().requires_grad_()
+    F.embedding(ids, w, scale_grad_by_freq=True).backward(dy)
+    m(ids).backward(dy)
+    torch.testing.assert_close(m.weight.grad, w.grad)
+    m, ids = _shared(device)
+    m.embedding.sparse = True
+    m(ids).backward(dy)
+    assert m.weight.grad.is_sparse
+    m, ids = _shared(device)
+    m.embedding.max_norm = 0.5
+    out = m(ids)
+    assert out.norm(dim=-1).le(0.5 * (1 + 1e-5)).all()
+    assert m.weight[[1, 5, 39, 0, 2]].norm(dim=-1).le(0.5 * (1 + 1e-5)).all() and m.weight[3].norm() > 1
+
+
+@pytest.mark.parametrize("device", DEVICES)
+def test_shared_embeddings_under_function_transforms_and_tracing(device):
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from torch._subclasses import FakeTensorMode
+
+    m, ids = _shared(device, scale=2.0)
+    want = m(ids).detach()
+    assert torch.equal(torch.vmap(m)(ids), want)
+    params = dict(m.named_parameters())
+    tangents = {k: torch.randn_like(p) for k, p in params.items()}
+
+    def f(p):
+        return torch.func.functional_call(m, p, (ids,))
+
+    grads = torch.func.grad(lambda p: f(p).sum())(params)
+    count = torch.bincount(ids.flatten(), minlength=40).to(want.dtype)
+    assert torch.equal(grads["embedding.weight"], (2 * count)[:, None].expand(40, 16))
+    out, tangent = torch.func.jvp(f, (params,), (tangents,))
+    assert torch.equal(out, want) and torch.equal(tangent, 2 * tangents["embedding.weight"][ids])
+    assert torch.equal(make_fx(m)(ids)(ids.flip(0)), want.flip(0))
+    assert torch.equal(torch.jit.trace(m, ids)(ids.flip(0)), want.flip(0))
+    assert torch.equal(torch.fx.symbolic_trace(m)(ids), want)
+    assert torch.equal(torch.jit.script(m)(ids), want)
+    with FakeTensorMode(allow_non_fake_inputs=True) as mode:
+        fake = m(mode.from_tensor(ids))
+    assert fake.shape == (2, 3, 16) and fake.device.type == device
