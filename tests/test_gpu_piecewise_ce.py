@@ -272,3 +272,16 @@ def test_cuda_refusals():
         ops.piecewise_linear_cross_entropy(h.float(), w.float(), t)
     with pytest.raises(RuntimeError, match="one CUDA device"):
         ops.piecewise_linear_cross_entropy(h, w, t.cpu())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("reduction", ["mean", "sum"])
+@pytest.mark.parametrize("up", [float("inf"), float("-inf"), float("nan")])
+def test_upstream_infinity_does_not_reach_rows_that_do_not_count(dtype, reduction, up):
+    """As in ``F.cross_entropy``: the gradient of an ignored row is 0 whatever arrives."""
+    h, w, t = _inputs(70, 300, 64, dtype, 13)
+    skip = t == -100
+    _, dh, dw = _run(h, w, t, reduction, torch.tensor(up, device="cuda"))
+    assert skip.any() and dh[skip].eq(0).all()
+    assert not dh[~skip].isfinite().any() and not dw.isfinite().all()
