@@ -88,8 +88,9 @@ __global__ void __launch_bounds__(256) join_tiles_kernel(const float2* __restric
 // then rounds an improbable target to exactly -1, where -1 times a weight that all rows
 // share would round the same way in every row (2-norm error of the gradients of a
 // 512 x 32000 bf16 mean 2.3e-3 instead of 1.9e-3).  A weight that is no number goes into
-// dz: in alpha it would meet the zeros of the rows that do not count (0 * inf).  f: the
-// power of two of fp16.
+// dz: in alpha it would meet the zeros of the rows that do not count (0 * inf), and as
+// the largest one it would leave the other rows without their scale.  f: the power of two
+// of fp16.
 __global__ void __launch_bounds__(1024) row_scale_kernel(const int64_t* __restrict__ targets, int64_t n, int64_t V,
                                                          int64_t ignore, const float* __restrict__ g, int g_per_row,
                                                          const float* __restrict__ factor, float f,
@@ -98,10 +99,12 @@ __global__ void __launch_bounds__(1024) row_scale_kernel(const int64_t* __restri
   float most = g_per_row ? 0.f : g[0] * factor[0];
   float inv = f, all = f;
   if (g_per_row) {  // every block finds it for itself
-    for (int64_t i = threadIdx.x; i < n; i += 1024)
-      if (counts(targets[i], ignore, V)) most = fmaxf(most, fabsf(g[i]));
+    for (int64_t i = threadIdx.x; i < n; i += 1024) {
+      const float a = fabsf(g[i]);
+      if (a < INFINITY && counts(targets[i], ignore, V)) most = fmaxf(most, a);
+    }
     most = block_max(most, red);
-    if (!(most > 1e-30f && most < INFINITY)) most = 1.f;  // nothing, or no number to divide by
+    if (!(most > 1e-30f)) most = 1.f;  // nothing, or too little to divide by
     inv = f / most;
   } else if (!(fabsf(most) < INFINITY)) {
     all = most;

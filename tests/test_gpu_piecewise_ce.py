@@ -285,3 +285,19 @@ def test_upstream_infinity_does_not_reach_rows_that_do_not_count(dtype, reductio
     _, dh, dw = _run(h, w, t, reduction, torch.tensor(up, device="cuda"))
     assert skip.any() and dh[skip].eq(0).all()
     assert not dh[~skip].isfinite().any() and not dw.isfinite().all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("bad", [float("inf"), float("-inf"), float("nan")])
+def test_a_weight_without_a_value_stays_in_its_row(dtype, bad):
+    """The other rows' dh has the bits that it has beside a finite weight."""
+    h, w, t = _inputs(70, 300, 64, dtype, 14)
+    t[:4] = torch.tensor([5, 6, 7, -100], device="cuda")
+    g = torch.full((70,), 50.0, device="cuda")
+    g[9:] += torch.rand(61, device="cuda", generator=torch.Generator("cuda").manual_seed(1))
+    _, want, _ = _run(h, w, t, "none", g)
+    g[0], g[3] = bad, bad
+    _, dh, dw = _run(h, w, t, "none", g)
+    assert torch.equal(dh[1:], want[1:]) and dh[3].eq(0).all()
+    assert not dh[0].isfinite().any() and not dw.isfinite().all()
