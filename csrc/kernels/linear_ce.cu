@@ -97,7 +97,7 @@ __global__ void __launch_bounds__(1024) row_scale_kernel(const int64_t* __restri
                                                          float* __restrict__ row_scale, float* __restrict__ alpha) {
   __shared__ float red[32];
   float most = g_per_row ? 0.f : g[0] * factor[0];
-  float inv = f, all = f;
+  float all = f;
   if (g_per_row) {  // every block finds it for itself
     for (int64_t i = threadIdx.x; i < n; i += 1024) {
       const float a = fabsf(g[i]);
@@ -105,13 +105,13 @@ __global__ void __launch_bounds__(1024) row_scale_kernel(const int64_t* __restri
     }
     most = block_max(most, red);
     if (!(most > 1e-30f)) most = 1.f;  // nothing, or too little to divide by
-    inv = f / most;
   } else if (!(fabsf(most) < INFINITY)) {
     all = most;
     most = 1.f;
   }
+  // the quotient: the largest weight times a rounded 1 / most would not always be f
   for (int64_t i = (int64_t)blockIdx.x * 1024 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 1024)
-    row_scale[i] = counts(targets[i], ignore, V) ? (g_per_row ? g[i] * inv : all) : 0.f;
+    row_scale[i] = counts(targets[i], ignore, V) ? (g_per_row ? f * (g[i] / most) : all) : 0.f;
   if (blockIdx.x == 0 && threadIdx.x == 0) alpha[0] = most / f;
 }
 

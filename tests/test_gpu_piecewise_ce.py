@@ -301,3 +301,16 @@ def test_a_weight_without_a_value_stays_in_its_row(dtype, bad):
     _, dh, dw = _run(h, w, t, "none", g)
     assert torch.equal(dh[1:], want[1:]) and dh[3].eq(0).all()
     assert not dh[0].isfinite().any() and not dw.isfinite().all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_any_one_weight_for_all_rows(dtype):
+    """``test_one_weight_for_all_rows`` at weights whose reciprocal times themselves is not
+    1 in fp32 (1 / 41 and about one number in seven)."""
+    h, w, t = _inputs(200, 900, 64, dtype, 21)
+    for weight in (1 / 41, 1 / 47, 1 / 55, 0.83):
+        g = torch.full((200,), weight, device="cuda")
+        _, dh, dw = _run(h, w, t, "none", g)
+        _, dh2, dw2 = _run(h, w, t, "sum", g[0])
+        assert torch.equal(dh, dh2) and torch.equal(dw, dw2)
