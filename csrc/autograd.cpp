@@ -188,7 +188,7 @@ at::Tensor piecewise_linear_ce(const at::Tensor& h, const at::Tensor& w, const a
     return t.stride(1) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 &&
                    t.stride(0) * (int64_t)t.element_size() % 16 == 0 && (t.stride(0) >= t.size(1) || t.size(0) <= 1)
                ? t
-               : t.contiguous();
+               : t.clone(at::MemoryFormat::Contiguous);  // a contiguous tensor may start anywhere
   };
   const at::Tensor h2 = rows16(h.dim() == 2 ? h : h.reshape({targets.numel(), w.size(1)})), w2 = rows16(w),
                    t = (targets.dim() == 1 ? targets : targets.reshape({-1})).contiguous();

@@ -314,3 +314,20 @@ def test_any_one_weight_for_all_rows(dtype):
         _, dh, dw = _run(h, w, t, "none", g)
         _, dh2, dw2 = _run(h, w, t, "sum", g[0])
         assert torch.equal(dh, dh2) and torch.equal(dw, dw2)
+
+
+@pytest.mark.gpu
+def test_contiguous_operands_that_start_anywhere():
+    """Contiguous h and w off a 16-byte boundary (slices of a flat buffer)."""
+    h, w, t = _inputs(33, 130, 24, torch.bfloat16, 15)
+    g = torch.tensor(1.0, device="cuda")
+    want = _run(h, w, t, "mean", g)
+
+    def moved(x, off):
+        flat = torch.empty(x.numel() + 8, device="cuda", dtype=x.dtype)
+        return flat[off:off + x.numel()].view(x.shape).copy_(x)
+
+    for off in (1, 4):
+        for a, b in ((moved(h, off), w), (h, moved(w, off)), (moved(h, off), moved(w, off))):
+            for x, y in zip(_run(a, b, t, "mean", g), want):
+                assert torch.equal(x, y)
