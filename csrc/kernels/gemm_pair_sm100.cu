@@ -1256,31 +1256,45 @@ void gemm_pair_ce_grad(const at::Tensor& H, const at::Tensor& W, const at::Tenso
 
 // K ranges that let a product of few tiles use every CTA pair: each of at least 8
 // k-blocks, all units in one wave.  1 where the tiles alone fill the pairs.
-int gemm_pair_slices(int64_t M, int64_t N, int64_t K, int dev) {
+static int slices_of(int64_t M, int64_t N, int64_t K, int64_t pairs) {
   const int64_t tiles = ((M + 2 * BM - 1) / (2 * BM)) * ((N + BN - 1) / BN), nk = (K + BK - 1) / BK;
-  return (int)std::max<int64_t>(1, std::min<int64_t>({max_pairs(dev) / std::max<int64_t>(tiles, 1), nk / 8, 64}));
+  return (int)std::max<int64_t>(1, std::min<int64_t>({pairs / std::max<int64_t>(tiles, 1), nk / 8, 64}));
 }
+int gemm_pair_slices(int64_t M, int64_t N, int64_t K, int dev) { return slices_of(M, N, K, max_pairs(dev)); }
 
-// Vocabulary rows at a time for the backward of the linear cross entropy, whose three
-// products a piece run in waves of one tile a CTA pair: the width whose waves cost
-// least over all pieces, among those whose 16-bit (n, width) buffer stays below `bytes`
-// (at least 1024 rows).  N = 16384, V = 32000, d = 2048: 4 pieces of 8192 rows leave the
-// 256 tiles of each piece's dw 13 % short of whole waves of 74; 5 of 6912 (216 tiles) 3 %.
+// Vocabulary rows at a time for the backward of the linear cross entropy: all of them
+// where their 16-bit (n, width) buffer stays below `bytes`, else a width of at least 1024
+// rows.  The three products of a piece run in waves of one tile a CTA pair, and a piece
+// adds its share of dh to the others'; narrower than the buffer allows where the sum of
+// these says 2 % or more (below that it decides no better than chance).  At most 33 widths
+// are looked at.
+//   backward, ms                     widest         chosen
+//   16384 x 32000 x 2048  bf16       8192: 5.09     6912: 4.94
+//   17238 x 32000 x 656   bf16       7680: 2.68     6144: 2.39
+//   11712 x 100287 x 472  fp16      11264: 4.49     9472: 4.10
+//   10000 x 50257 x 768   fp16      13312: 2.43    12544: 2.28
+// Of 27 sizes between 1500 and 60000 rows whose least sum was not the widest piece, it was
+// faster in 18, by up to 12 %, and slower in 5, by up to 4 %.
 int64_t gemm_pair_ce_piece(int64_t n, int64_t V, int64_t d, int64_t bytes, int dev) {
-  const int64_t pairs = max_pairs(dev);
   const auto up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
-  const int64_t tm = up(n, 256), td = up(d, 256), most = std::max<int64_t>(4, std::min(up(V, 256), bytes / (512 * std::max<int64_t>(n, 1))));
-  // the time of a launch in steps of one K element of a tile (6 ns)
-  constexpr int64_t kLaunch = 1000;
+  const int64_t tiles = up(V, 256), most = std::max<int64_t>(4, std::min(tiles, bytes / (512 * std::max<int64_t>(n, 1))));
+  if (most >= tiles) return 256 * tiles;
+  const int64_t pairs = max_pairs(dev), tm = up(n, 256), td = up(d, 256);
+  // times in steps of one K element of a tile (6 ns, in which DRAM moves 39 KB): three
+  // launches, and dh in fp32 read and written
+  const int64_t fixed = 3000 + n * d * 8 / 39000;
   const auto cost = [&](int64_t w) {
-    const int64_t tv = up(w, 256), sh = gemm_pair_slices(n, d, w, dev), sw = gemm_pair_slices(w, d, n, dev);
-    return up(tm * tv, pairs) * d + up(tm * td * sh, pairs) * up(w, sh) + up(tv * td * sw, pairs) * up(n, sw) + 3 * kLaunch;
+    const int64_t tv = up(w, 256), sh = slices_of(n, d, w, pairs), sw = slices_of(w, d, n, pairs);
+    return up(tm * tv, pairs) * d + up(tm * td * sh, pairs) * up(w, sh) + up(tv * td * sw, pairs) * up(n, sw) + fixed;
   };
-  int64_t best = most, least = -1;
-  for (int64_t r = most; r >= std::max<int64_t>(4, most / 4); --r) {
+  const auto total = [&](int64_t r) {
     const int64_t w = 256 * r, full = V / w, last = V - full * w;
-    const int64_t c = full * cost(w) + (last > 0 ? cost(last) : 0);
-    if (least < 0 || c < least) least = c, best = r;
+    return full * cost(w) + (last > 0 ? cost(last) : 0);
+  };
+  int64_t best = most, least = total(most) / 51 * 50;
+  for (int64_t r = most, step = std::max<int64_t>(1, most / 32); r >= std::max<int64_t>(4, most / 4); r -= step) {
+    const int64_t c = total(r);
+    if (c < least) least = c, best = r;
   }
   return 256 * best;
 }

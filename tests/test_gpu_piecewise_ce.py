@@ -331,3 +331,11 @@ def test_contiguous_operands_that_start_anywhere():
         for a, b in ((moved(h, off), w), (h, moved(w, off)), (moved(h, off), moved(w, off))):
             for x, y in zip(_run(a, b, t, "mean", g), want):
                 assert torch.equal(x, y)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("N,V", [(40000, 5003), (140000, 1500), (1, 100287), (3, 9)])
+def test_default_pieces(N, V):
+    """The default width where its buffer takes the vocabulary in two pieces, and in one."""
+    h, w, t = _inputs(N, V, 16, torch.bfloat16, 16)
+    _compare(h, w, t, "sum", torch.tensor(1.0, device="cuda"))
