@@ -42,10 +42,13 @@ def ntp_objective(models: Dict[str, nn.Module], ctx: TrainingContext, batch: Any
     input_ids = batch["input_ids"]
     if input_ids.device != device:
         input_ids = input_ids.to(device, non_blocking=True)
-    if batch.get("fused_lm_loss", False):  # extension: chunked head + CE, no full logits
+    fused = batch.get("fused_lm_loss", False)
+    if isinstance(fused, str) and fused not in ("", "rows", "pieces"):
+        raise ValueError(f"fused_lm_loss must be a truth value, 'rows' or 'pieces', got {fused!r}")
+    if fused:  # extension: chunked head + CE, no full logits
         targets = torch.cat([input_ids[:, 1:], input_ids.new_full((input_ids.shape[0], 1), -100)], dim=1)
         # "pieces": in pieces of the vocabulary instead of chunks of rows
-        how = {"lm_loss": "pieces"} if batch["fused_lm_loss"] == "pieces" else {}
+        how = {"lm_loss": "pieces"} if isinstance(fused, str) and fused == "pieces" else {}
         out = model(input_ids, labels=targets, **how)
         loss = out["lm_loss"]
     else:

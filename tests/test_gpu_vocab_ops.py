@@ -342,3 +342,22 @@ def test_losses_refuse_forward_mode():
     with fw.dual_level():  # the teacher is a constant in both modes
         loss = ops.topk_distillation(x, fw.make_dual(teacher, torch.ones_like(teacher)), tids)
         assert fw.unpack_dual(loss).tangent is None and torch.equal(loss, ops.topk_distillation(x, teacher, tids))
+
+
+@pytest.mark.parametrize("how", ["piece", "chunks", ""])
+def test_unknown_kind_of_fused_loss_is_refused(how):
+    """A misspelt kind is an error; the empty string means off, as any false value does."""
+    from genesis.model.hlrt import HLRT
+    from genesis.training.train_phase1_bootstrap import ntp_objective
+    from llm_research_b200.models.presets import build_hlrt_config
+
+    cfg = build_hlrt_config("toy")
+    torch.manual_seed(0)
+    m = HLRT(cfg)
+    ids = torch.randint(0, cfg.vocab_size, (1, 16), generator=torch.Generator().manual_seed(1))
+    batch = {"input_ids": ids, "fused_lm_loss": how}
+    if how == "":
+        assert torch.isfinite(ntp_objective({"hlrt": m}, None, batch))
+    else:
+        with pytest.raises(ValueError, match="fused_lm_loss"):
+            ntp_objective({"hlrt": m}, None, batch)
