@@ -322,6 +322,27 @@ __global__ void __launch_bounds__(kThreads, (kFwdBlocks<T, W>))
     }
   }
   const float m = ms.x;
+  float rest = fmaf(-m, k2, base_of(m, k2));  // the rounding of the base
+  if (fabsf(m) > far_limit(k2) && fabsf(m) < INFINITY) {  // differences to m first: the row again, by every warp
+    float s = 0.f;
+    const auto one = [&](int i) { s += fast_exp2((to_f(x[i]) - m) * k2); };
+    const auto vec = [&](int, const uint4& v) {
+#pragma unroll
+      for (int j = 0; j < Pairs<T>::N; ++j) {
+        const float2 f = f2_unpack(Pairs<T>::get(v, j));
+        s += fast_exp2((f.x - m) * k2) + fast_exp2((f.y - m) * k2);
+      }
+    };
+    walk<2>(x, V, tid, 32 * W, one, [&](int, int, const uint4 (&v)[2]) { vec(0, v[0]), vec(0, v[1]); }, vec);
+    ms.y = warp_sum(s);
+    if constexpr (W > 1) {
+      __syncthreads();  // `part` has been read
+      if (lane == 0) part[warp].y = ms.y;
+      __syncthreads();
+      ms.y = warp_sum(lane < kWarps ? part[lane].y : 0.f);
+    }
+    rest = 0.f;
+  }
 
   Entries e{-INFINITY, 0.f, 0.f, 0.f};
   if (W == 1 || warp * 32 < t.K) {
@@ -365,13 +386,6 @@ __global__ void __launch_bounds__(kThreads, (kFwdBlocks<T, W>))
     }
   }
   if (W > 1 && warp != 0) return;
-  float rest = fmaf(-m, k2, base_of(m, k2));  // the rounding of the base
-  if (fabsf(m) > far_limit(k2) && fabsf(m) < INFINITY) {  // differences to m first (this warp alone, the whole row)
-    float s = 0.f;
-    for (int i = lane; i < V; i += 32) s += fast_exp2((to_f(x[i]) - m) * k2);
-    ms.y = warp_sum(s);
-    rest = 0.f;
-  }
   if (lane == 0) {
     const float log2_s = log2f(ms.y);
     stats[row] = RowStats{base_of(m, k2), log2_s, m, some ? 1.f : 0.f};
@@ -474,13 +488,15 @@ __global__ void __launch_bounds__(kThreads, (kBwdBlocks<T, W>))
   for (int i = tid; i < size; i += G) seen[i] = -1;
 
   const T* xp = x + c0;
-  if ((reinterpret_cast<uintptr_t>(xp) & 15) == (reinterpret_cast<uintptr_t>(dp) & 15) && !far) {
+  if ((reinterpret_cast<uintptr_t>(xp) & 15) == (reinterpret_cast<uintptr_t>(dp) & 15)) {
     const uint64_t kk = f2_pack(k2, k2), nb = f2_pack(-base, -base), nl = f2_pack(-l2, -l2), cc = f2_pack(coef, coef);
-    const auto vec = [&](int i, const uint4& v) {
+    const auto put = [&](auto is_far, int i, const uint4& v) {
       uint32_t o[4];
 #pragma unroll
       for (int j = 0; j < Pairs<T>::N; ++j) {
-        const float2 e = f2_unpack(f2_add(f2_fma(Pairs<T>::get(v, j), kk, nb), nl));
+        const uint64_t xx = Pairs<T>::get(v, j);
+        const float2 e = f2_unpack(f2_add(decltype(is_far)::value ? f2_mul(f2_add(xx, f2_pack(-m, -m)), kk)
+                                                                  : f2_fma(xx, kk, nb), nl));
         const float2 r = f2_unpack(f2_mul(f2_pack(fast_exp2(e.x), fast_exp2(e.y)), cc));
         if constexpr (sizeof(T) == 4) {
           o[2 * j] = __float_as_uint(r.x);
@@ -491,14 +507,18 @@ __global__ void __launch_bounds__(kThreads, (kBwdBlocks<T, W>))
       }
       *reinterpret_cast<uint4*>(dp + i) = make_uint4(o[0], o[1], o[2], o[3]);
     };
-    constexpr int U = kBwdU<T, W>;
-    walk<U>(
-        xp, len, tid, G, [&](int i) { dp[i] = from_f<T>(coef * q(to_f(xp[i]))); },
-        [&](int i, int step, const uint4 (&v)[U]) {
+    const auto run = [&](auto is_far, auto unroll) {
+      constexpr int U = decltype(unroll)::value;
+      walk<U>(
+          xp, len, tid, G, [&](int i) { dp[i] = from_f<T>(coef * q(to_f(xp[i]))); },
+          [&](int i, int step, const uint4 (&v)[U]) {
 #pragma unroll
-          for (int u = 0; u < U; ++u) vec(i + u * step, v[u]);
-        },
-        vec);
+            for (int u = 0; u < U; ++u) put(is_far, i + u * step, v[u]);
+          },
+          [&](int i, const uint4& v) { put(is_far, i, v); });
+    };
+    if (!far) run(std::false_type{}, std::integral_constant<int, kBwdU<T, W>>{});
+    else run(std::true_type{}, std::integral_constant<int, 2>{});
   } else {
     for (int i = tid; i < len; i += G) dp[i] = from_f<T>(coef * q(to_f(xp[i])));
   }
