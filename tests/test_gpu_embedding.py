@@ -378,3 +378,20 @@ def test_shared_embeddings_under_function_transforms_and_tracing(device):
     with FakeTensorMode(allow_non_fake_inputs=True) as mode:
         fake = m(mode.from_tensor(ids))
     assert fake.shape == (2, 3, 16) and fake.device.type == device
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,V,d", [(5000, 300000, 16), (40000, 300000, 8), (40000, 262145, 33)])
+def test_sort_of_three_passes_over_several_blocks(dtype, n, V, d):
+    from llm_research_b200 import ops
+
+    g = torch.Generator().manual_seed(n + V)
+    ids = _tokens(n, V, g)
+    ids[::7] = ids[0] % 1000 + 511 * 512  # tokens that differ in the last digit alone
+    ids, w = ids.cuda(), torch.zeros(V, d, device="cuda", dtype=dtype, requires_grad=True)
+    dy = torch.randn(n, d, generator=g).to(dtype).cuda()
+    dw, = torch.autograd.grad(ops.embedding(ids, w), w, dy)
+    _check_grad(dw, dy, ids, V, 1.0)
+    dw2, = torch.autograd.grad(ops.embedding(ids, w), w, dy)
+    assert torch.equal(dw, dw2)

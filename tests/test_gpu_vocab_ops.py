@@ -361,3 +361,25 @@ def test_unknown_kind_of_fused_loss_is_refused(how):
     else:
         with pytest.raises(ValueError, match="fused_lm_loss"):
             ntp_objective({"hlrt": m}, None, batch)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_each_operator_gives_the_same_bits_again(dtype):
+    """Every sum has a fixed order.  (In the whole step autograd's own products come between.)"""
+    from llm_research_b200 import ops
+
+    ids, w, mix, targets, teacher, tids = _inputs("cuda", dtype, N=3000, V=5003)
+    h = w[ids].clone()
+    x = (h.float() @ w.float().t()).to(dtype)
+
+    def run():
+        a, b, c = (t.detach().clone().requires_grad_() for t in (w, h, x))
+        out = ops.embedding(ids, a, 8.0)
+        ce = ops.piecewise_linear_cross_entropy(b, a, targets, piece=1024)
+        kd = ops.topk_distillation(c, teacher, tids, 2.0)
+        return (out, ce, kd, *torch.autograd.grad(out, a, h), *torch.autograd.grad(ce, (b, a)),
+                *torch.autograd.grad(kd, c))
+
+    for u, v in zip(run(), run()):
+        assert torch.equal(u, v)
