@@ -38,8 +38,9 @@ def _plain(x, teacher, ids, T, reduction):
     V = x.shape[-1]
     f = torch.float64 if x.dtype == torch.float64 else torch.float32
     x, teacher = x.to(f) / T, teacher.detach().to(f)
-    kept = (ids >= 0) & (ids < V) & (teacher != -math.inf)
+    kept = (ids >= 0) & (ids < V) & (teacher != -math.inf)  # what stands in padding is not looked at,
     some = kept.any(dim=-1)
+    x = torch.where(some[:, None], x, torch.zeros_like(x))  # nor what a row without entries holds
     y = torch.where(kept, teacher / T, torch.full_like(teacher, -math.inf))
     y = torch.where(some[:, None], y, torch.zeros_like(y))
     p = torch.where(kept, torch.softmax(y, dim=-1), torch.zeros_like(y))

@@ -368,3 +368,19 @@ def test_temperature_that_leaves_fp32_is_refused_on_cuda():
     for T in (1e-46, 1e-20, 1e20, 1e39):
         with pytest.raises(ValueError, match="temperature"):
             ops.topk_distillation(x, teacher, ids, T)
+
+
+def test_cpu_rows_without_a_teacher_do_not_look_at_the_logits():
+    """Loss 0 and gradient 0 there, as on CUDA, whatever the logits hold."""
+    from llm_research_b200 import ops
+
+    x, teacher, ids = _inputs(4, 31, 5, torch.float32, 3, ragged=False, device="cpu")
+    ids[1], teacher[2] = -1, float("-inf")
+    x[1, 3], x[2, 4] = float("nan"), float("inf")
+    x[3, 30] = float("-inf")
+    ids[3].clamp_(max=29)
+    for reduction in ("mean", "sum", "none"):
+        y = x.clone().requires_grad_()
+        loss = ops.topk_distillation(y, teacher, ids, 1.0, reduction)
+        dx, = torch.autograd.grad(loss.sum(), y)
+        assert loss.isfinite().all() and dx.isfinite().all() and dx[1:3].eq(0).all()
