@@ -37,10 +37,11 @@ MIN_TEMPERATURE, MAX_TEMPERATURE = 1e-18, 1e18
 def _plain(x, teacher, ids, T, reduction):
     V = x.shape[-1]
     f = torch.float64 if x.dtype == torch.float64 else torch.float32
-    x, teacher = x.to(f) / T, teacher.detach().to(f)
+    x, teacher = x.to(f), teacher.detach().to(f)
     kept = (ids >= 0) & (ids < V) & (teacher != -math.inf)  # what stands in padding is not looked at,
     some = kept.any(dim=-1)
     x = torch.where(some[:, None], x, torch.zeros_like(x))  # nor what a row without entries holds
+    x = (x - x.amax(dim=-1, keepdim=True).detach()) / T
     y = torch.where(kept, teacher / T, torch.full_like(teacher, -math.inf))
     y = torch.where(some[:, None], y, torch.zeros_like(y))
     p = torch.where(kept, torch.softmax(y, dim=-1), torch.zeros_like(y))

@@ -384,3 +384,15 @@ def test_cpu_rows_without_a_teacher_do_not_look_at_the_logits():
         loss = ops.topk_distillation(y, teacher, ids, 1.0, reduction)
         dx, = torch.autograd.grad(loss.sum(), y)
         assert loss.isfinite().all() and dx.isfinite().all() and dx[1:3].eq(0).all()
+
+
+@pytest.mark.parametrize("T", [0.25, 1.0])
+def test_cpu_row_of_the_lowest_value(T):
+    """Uniform, also where the value over T leaves fp32."""
+    from llm_research_b200 import ops
+
+    x, teacher, ids = _inputs(2, 31, 5, torch.float32, 3, ragged=False, device="cpu")
+    x[1] = 0.0
+    want = ops.topk_distillation(x, teacher, ids, T, "none")
+    x[1] = torch.finfo(torch.float32).min
+    torch.testing.assert_close(ops.topk_distillation(x, teacher, ids, T, "none"), want)
