@@ -25,11 +25,14 @@
 // (6.5 TB/s): its exponentials keep the special-function pipe 71 % busy and every row
 // ends in a join; moving a quarter of the exponentials to the FMA pipe did not help.
 #include "../common.cuh"
+#include "sm100.cuh"
 
 #include <cmath>
 
 namespace lrb {
 namespace {
+
+using namespace sm100;
 
 constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kPerThread = 4;                   // teacher entries a thread holds
@@ -182,26 +185,16 @@ __device__ __forceinline__ float2 warp_join(float2 v, float k2) {
   return make_float2(m, warp_sum(v.y * fast_exp2(base_of(v.x, k2) - base_of(m, k2))));
 }
 
-__device__ __forceinline__ unsigned cluster_rank() {
-  unsigned r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ unsigned cluster_size() {
-  unsigned r;
-  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
-  return r;
-}
 __device__ __forceinline__ void cluster_barrier() {
   __syncthreads();  // the aligned forms want converged warps
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  cluster_sync();
 }
 __device__ __forceinline__ float2 ld_peer(const float2* p, unsigned rank) {
-  const uint32_t a = (uint32_t)__cvta_generic_to_shared(p);
-  uint32_t q;
   float2 v;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(q) : "r"(a), "r"(rank));
-  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(q) : "memory");
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];"
+               : "=f"(v.x), "=f"(v.y)
+               : "r"(mapa_shared(smem_addr(p), rank))
+               : "memory");
   return v;
 }
 
@@ -277,7 +270,7 @@ __global__ void __launch_bounds__(kThreads, (kFwdBlocks<T, W>))
   __shared__ float2 part[kWarps], mine;
   __shared__ Entries entries[kWarps];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const unsigned rank = W == 1 ? 0 : cluster_rank(), split = W == 1 ? 1 : cluster_size();
+  const unsigned rank = W == 1 ? 0 : cluster_ctarank(), split = W == 1 ? 1 : cluster_nctarank();
   const int64_t row = W == 1 ? (int64_t)blockIdx.x * kWarps + warp : blockIdx.x / split;
   if (row >= n) return;  // W = 1 only: whole warps
   const T* x = row_ptr(logits, rows, row);

@@ -10,9 +10,12 @@
 //
 // Ids outside [0, V) give a row of NaN and no gradient; nothing is read for them.
 #include "../common.cuh"
+#include "sm100.cuh"
 
 namespace lrb {
 namespace {
+
+using namespace sm100;
 
 // ------------------------------------------------------------------ lookup
 // A copy: bounded by the bytes of the looked-up rows and the output (65520 x 4096 bf16
@@ -82,25 +85,13 @@ constexpr int kSortThreads = 1024;
 constexpr int kSortWarps = kSortThreads / 32;
 constexpr int kBatch = 8;  // keys a lane holds at a time
 
-__device__ __forceinline__ unsigned cluster_rank() {
-  unsigned r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
-__device__ __forceinline__ unsigned cluster_size() {
-  unsigned r;
-  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
-  return r;
-}
 __device__ __forceinline__ void cluster_barrier() {
   __syncthreads();  // the aligned forms want converged warps
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  cluster_sync();
 }
 __device__ __forceinline__ int ld_peer(const int* p, unsigned rank) {
-  uint32_t q;
   int v;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(q) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
-  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(q) : "memory");
+  asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(mapa_shared(smem_addr(p), rank)) : "memory");
   return v;
 }
 
@@ -138,7 +129,7 @@ template <typename IdT>
 __global__ void __launch_bounds__(kSortThreads, 1) sort_tokens_kernel(const IdT* __restrict__ ids, SortArgs a) {
   extern __shared__ int smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int rank = (int)cluster_rank(), blocks = (int)cluster_size();
+  const int rank = (int)cluster_ctarank(), blocks = (int)cluster_nctarank();
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int n = a.n, V = a.V, bits = a.bits;
   const int bins = 1 << bits;
