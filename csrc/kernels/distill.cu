@@ -19,11 +19,14 @@
 // Rows whose maximum is itself beyond F (rows that hold nothing but a mask, or a huge
 // offset) take differences x - m first, in a second walk of the forward.
 //
-// Bounded by the bytes of the logits: 16384 x 32000 bf16 with 64 entries forward 196 to
-// 204 us (5.1 to 5.4 TB/s) and backward 317 us (6.6 TB/s), 4093 x 100287 fp32 with 200 entries 261 us
-// and 559 us (6.3 and 5.9 TB/s).  The 16-bit forward is the furthest from the copy rate
-// (6.5 TB/s): its exponentials keep the special-function pipe 71 % busy and every row
-// ends in a join; moving a quarter of the exponentials to the FMA pipe did not help.
+// Bounded by the bytes of the logits: 16384 x 32000 bf16 with 64 entries forward 195 us
+// (5.4 TB/s) and backward 317 to 334 us (6.3 to 6.6 TB/s), 4093 x 100287 fp32 with 200
+// entries 256 to 261 us and 559 to 590 us (6.3 to 6.4 and 5.6 to 5.9 TB/s).  The 16-bit
+// forward is the furthest from the copy rate (6.5 TB/s): no unit is at its limit (special
+// functions 71 % busy, issue slots and DRAM 58 %; a quarter of the exponentials on the FMA
+// pipe made it slower), its loads run dry at the end of each row, which a block takes in
+// four steps, joins and leaves.  Rows beyond the limit are read twice in the forward:
+// 16384 x 32000 bf16 of them 312 and 377 us.
 #include "../common.cuh"
 #include "sm100.cuh"
 

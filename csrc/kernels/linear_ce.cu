@@ -11,17 +11,24 @@
 // and dz^T h (rows of dw, complete after one piece).  So 2NVd operations forward,
 // 6NVd backward, bounded by the tensor cores; the only (N, piece) array is dz.
 // N = 16384, V = 32000, d = 2048 bf16: forward 1.49 ms (1.44 PFLOP/s), the three
-// products of the backward 1.60, 1.49 and 1.49 ms in 5 pieces, the step 6.8 ms under the
-// power cap (1.26 PFLOP/s; cuBLAS products alone sustain 1.37).
+// products of the backward 1.60, 1.49 and 1.49 ms in 5 pieces, the step 6.8 to 6.9 ms under
+// the power cap (1.26 PFLOP/s; cuBLAS products alone sustain 1.37).  The loss by chunks of
+// rows, which keeps 16-bit logits and forms 6NVd, needs 6.3 ms there and 1.8 GB beside the
+// results instead of 0.5.
 //
-// The logits are the tensor cores' fp32 accumulators: against 64 bits the row losses are
-// off by 2-norm 4.6e-7 at d = 1024 and 1.8e-6 at d = 4096 (2.5e-7 and 5.7e-7 with fp32
-// multiply-adds), the accumulation cutting off what does not fit.
+// The logits are the tensor cores' fp32 accumulators, which cut off what does not fit:
+// against 64 bits the row losses are off by 2-norm 4.6e-7 at d = 1024 and 1.8e-6 at
+// d = 4096 (2.5e-7 and 5.7e-7 with fp32 multiply-adds).  Cutting off has one direction
+// (logits of targets are large and come out too small), so the error of a mean is no
+// smaller: +3e-7 of it at d = 1024, +6e-7 at 2048, +1.2e-6 at 4096.
 //
 // dz is the one value that is rounded to 16 bits on the way: it is an operand of
-// the two gradient products, relative 2^-9 (bf16) or 2^-12 (fp16) an element.  For
-// fp16, whose smallest normal number is 6e-5, it is scaled so that the largest |r_n| is
-// 2^13 and the products are scaled back.
+// the two gradient products, relative 2^-9 (bf16) or 2^-12 (fp16) an element.  With one
+// weight for all rows the gradients' error is 1.1 (bf16) to 1.4 times (fp16) that of their
+// own rounding.  For fp16, whose smallest normal number is 6e-5, dz is scaled so that the
+// largest finite |r_n| is 2^13 and the products are scaled back; a probability times its
+// row's weight below 2^-27 of that largest weight falls among the subnormals (an absolute
+// error of 2^-38 of it).
 #include "../common.cuh"
 
 #include <climits>
@@ -215,7 +222,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> linear_ce_fwd(const a
 
 // (dh, dw), each empty where it is not asked for.  `g` fp32: one value for each row,
 // or a single one that is multiplied by `factor`.  `piece`: vocabulary rows at a time, a
-// multiple of 8; 0: a buffer of at most 256 MB or 1024 rows.
+// multiple of 8; 0: gemm_pair_ce_piece's, of a buffer of at most 256 MB or 1024 rows.
 std::tuple<at::Tensor, at::Tensor> linear_ce_bwd(const at::Tensor& h, const at::Tensor& w, const at::Tensor& targets,
                                                  int64_t ignore, const at::Tensor& stats, const at::Tensor& g,
                                                  bool g_per_row, const at::Tensor& factor, int64_t piece, bool need_h,

@@ -12,12 +12,15 @@ row without entries has loss 0, gradient 0 and is left out of the mean.  A token
 listed twice has the sum of its probabilities.  The teacher gets no gradient.
 On CUDA the loss can be differentiated once, in reverse mode (anything else raises).
 
-CUDA (``csrc/kernels/distill.cu``): the forward reads the logits once and keeps
+CUDA (``csrc/kernels/distill.cu``): the forward reads the logits once (twice where a
+row's largest value is beyond some 2.9e6 ``T`` either way) and keeps
 four numbers a row and the teacher's probabilities; the backward reads them once and writes the gradient; fp32
 arithmetic for bf16, fp16 and fp32 logits: a row's loss is off by some ``T^2 2^-20``
 times the sizes of its logarithms, which is much beside the loss itself once ``T``
-flattens both distributions (hundreds).  The full-vocabulary form of the
-same loss is ``VerificationDistillation.temperature_scaled_loss``.
+flattens both distributions (hundreds).  The full-vocabulary form is
+``VerificationDistillation.temperature_scaled_loss``, which divides by the first
+dimension: on ``(N, V)`` logits it is the mean of all tokens listed, on ``(B, S, V)``
+it is ``S`` times that.
 """
 
 from __future__ import annotations

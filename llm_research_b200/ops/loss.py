@@ -19,12 +19,19 @@ target logit are combined over the group, and the gradients come back
 replicated (``dh`` summed over the shards, ``dW`` gathered from them).
 
 :func:`piecewise_linear_cross_entropy` is the head + loss in pieces of the
-*vocabulary*: no logits are kept, or rounded.  :func:`linear_cross_entropy` walks
+*vocabulary*: no logits are kept, and the loss comes from their fp32 values.  Their
+gradient is rounded to the operands' 16-bit type once, as an operand of the two
+gradient products.  :func:`linear_cross_entropy` walks
 over rows, keeps 16-bit logits of a chunk of rows and forms the gradients in the
 forward (three products); the piecewise form needs the products of the backward
 only when a backward comes (one product forward, three backward: the logits are
 formed twice), takes per-row losses and weights, and its working memory is
-``N * piece`` values whatever the vocabulary.
+``N * piece`` values whatever the vocabulary.  Which one (mean and both gradients):
+by rows is 9 to 11 % faster on large products of an aligned vocabulary (16384 x 32000
+x 2048 bf16: 6.3 ms and 1.8 GB, in pieces 6.9 ms and 0.5 GB); in pieces is faster for
+short batches (512 x 32000 x 256: 107 us against 335), for a vocabulary that is no
+multiple of 8 (4093 x 100287 x 1024 fp16: 2.6 ms against 18.6), and for losses alone,
+and its gradients are nearer to the 64-bit ones (1.9e-3 against 3.1e-3 in bf16).
 """
 
 from __future__ import annotations
@@ -154,7 +161,8 @@ def piecewise_linear_cross_entropy(h: torch.Tensor, w: torch.Tensor, targets: to
     leading shape, 0 in rows that do not count), fp32.  CUDA: bf16 or fp16, ``d`` a
     multiple of 8, on the CTA-pair tensor-core kernel (``csrc/kernels/linear_ce.cu``):
     the log-sum-exp is taken from the fp32 products, and the backward forms the
-    logits' gradient for ``piece`` vocabulary rows at a time (default: a buffer of
+    logits' gradient, rounded to the operands' type (fp16: scaled by the largest row
+    weight), for ``piece`` vocabulary rows at a time (default: a buffer of
     at most 256 MB, or 1024 rows).  As in any matrix product, an ``inf`` or NaN in a row of ``h``
     that does not count still reaches ``dw`` (0 * inf).  On CUDA the loss can be
     differentiated once, in reverse mode (anything else raises)."""
